@@ -26,6 +26,8 @@ extern "C" {
 #define MI355_DT_BF16 0
 #define MI355_DT_FP16 1
 #define MI355_DT_FP8_E4M3FN 2 /* OCP e4m3fn (gfx950 native); KV cache only */
+#define MI355_DT_FP32 3       /* norm weights and rotation tables of mi355_qk_norm_rope_append() only */
+#define MI355_DT_FP4_E2M1 4   /* OCP e2m1 codes with a power-of-two scale byte (e8m0) per 32 elements; KV cache only */
 
 /* kernel selection for mi355_gqa_paged_decode(): which implementation serves the call */
 #define MI355_KERNEL_AUTO 0    /* MFMA kernel when the shape qualifies, else the generic one */
@@ -268,6 +270,105 @@ int mi355_kv_append_fp8(const void* x_new, void* cache, float* scale, const int3
 int mi355_prefill_input_facts(const int32_t* cu_seqlens_q, const int32_t* cache_seqlens, const int32_t* block_table,
                               int64_t bt_row_stride, const float* k_scale, const float* v_scale, int batch,
                               int max_pages_per_req, int32_t* facts, void* hip_stream);
+
+/*
+ * The 4-bit KV cache of the entry points below (no counterpart in the reference, whose caches are 16-bit or FP8).  32
+ * consecutive head elements form a block: e2m1 codes, two to a byte with the lower nibble first, and one scale byte,
+ * x = code * 2^(byte - 127) (OCP microscaling; byte 255 makes the block NaN).  Layout, pages of page_size tokens:
+ *   codes  [n_pages, heads_kv, page_size, dim / 2]  bytes       scales [n_pages, heads_kv, page_size, dim / 32]  bytes
+ * i.e. the rows of one (page, kv head) are contiguous.  Slot s = token s % page_size of page s / page_size, as in the
+ * token-major pools above.  Rounding: byte - 127 is the smallest e >= -126 with max|x| <= 6 * 2^e, codes go to the nearest
+ * value, ties to the even code; a block that holds an infinity or NaN gets byte 255 (all codes 0); magnitudes above
+ * 3 * 2^126 are stored as that.
+ */
+
+/*
+ * Pages for the new tokens of a step, taken from a list of free pages, and where each token goes.
+ *
+ *   cached         [batch] int32: tokens of each sequence before the step
+ *   cu_seqlens_q   [batch + 1] int32, non-decreasing: sequence b has the new tokens [cu[b], cu[b+1]) of the packed step; NULL:
+ *                  one new token per sequence (total_q == batch)
+ *   block_table    [batch, >= max_pages] int32, row stride bt_row_stride: entries of the pages taken are written, no other
+ *   free_pages     [n_pages] int32, a stack: the free pages are free_pages[0 .. free_count[0]), taken from the end
+ *   free_count     [1] int32 (read as if clamped to [0, n_pages])
+ * Sequence b, with c = cached[b] and n new tokens, needs ceil((c + n) / page_size) - ceil(c / page_size) pages.  Sequences are
+ * served in batch order; one is refused if it would outgrow its row (max_pages * page_size tokens, or 2^31 - 1), if c < 0, or if the
+ * pages that it and all earlier sequences (that fit their rows) need are more than there are and it needs any.  Page i of the
+ * call, counted in batch order and then by logical page, is free_pages[free - 1 - i].
+ *   slots          [total_q] int64: page * page_size + offset of each new token; -1 for tokens of refused sequences and tokens that
+ *                  belong to no sequence (a padded step)
+ *   positions      [total_q] int32: position of each token in its sequence, -1 likewise
+ *   seqlens_out    [batch] int32: c + n for a served sequence, else c
+ *   refused        [batch] bytes: 1 for a sequence with new tokens that was not served
+ *   free_count_out [1] int32: pages left.  free_count itself and free_pages are not written, so the same call again gives
+ *                  the same answer; the caller passes free_count_out on.  It must not be free_count's memory.
+ */
+int mi355_kv_alloc(const int32_t* cached, const int32_t* cu_seqlens_q, int32_t* block_table, int64_t bt_row_stride, int max_pages,
+                   const int32_t* free_pages, const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* seqlens_out,
+                   uint8_t* refused, int32_t* free_count_out, int batch, int total_q, int page_size, int n_pages, void* hip_stream);
+
+/*
+ * Pages of finished sequences back onto the list: the ceil(seqlens[b] / page_size) first entries of each finished sequence's
+ * row (at most max_pages), in batch order, go to free_pages[free_count ..); places past n_pages are not written.
+ *   finished       [batch] bytes, not 0 = finished
+ *   seqlens_out    [batch] int32: 0 for finished sequences, else seqlens[b]
+ *   free_count_out [1] int32: free_count plus the pages returned, at most n_pages; not free_count's memory
+ */
+int mi355_kv_release(const uint8_t* finished, const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride, int max_pages,
+                     int32_t* free_pages, const int32_t* free_count, int32_t* seqlens_out, int32_t* free_count_out, int batch,
+                     int page_size, int n_pages, void* hip_stream);
+
+/*
+ * RMS norm of query and key rows per head, rotary position embedding, and the append of keys and values to the cache, in one
+ * pass.  For every token t and head:
+ *   y = x * weight / sqrt(mean(x^2) + eps)              (q_weight / k_weight NULL: y = x; values are never normed)
+ *   the first rotary_dim elements of y are rotated by the angle of positions[t]: pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if
+ *   interleaved, i < rotary_dim / 2:  (a cos - b sin, b cos + a sin) with row positions[t] of the tables
+ * Query rows go to q_out, rounded once to x_dtype.  Key rows (and value rows as they came) go to slot slots[t] of the cache:
+ *   16-bit cache (cache_dtype == x_dtype)  [n_phys_tokens, heads_kv, dim], rounded once
+ *   FP8 cache                              the same with k_scale, v_scale [n_phys_tokens, heads_kv] fp32: the format and rounding
+ *                                          of mi355_kv_append_fp8()
+ *   4-bit cache                            as above, k_scale, v_scale = the scale bytes
+ * Norm and rotation are formed in fp32; keys that become codes in fp64, rounded to fp32 once and then to the code, so that codes do
+ * not depend on the order of a sum.  Tokens whose slot is outside the pool are not appended (their query row is still written).
+ *   q, k, v        rows of dim elements, heads dim apart, tokens *_stride elements apart (slices of one projection qualify); 4-byte
+ *                  aligned with even strides
+ *   weight_dtype   x_dtype or MI355_DT_FP32; table_dtype likewise
+ *   cos_table,
+ *   sin_table      [max_position, rotary_dim / 2] (NULL with rotary_dim 0); positions outside are read as the nearest row
+ *   positions      [tokens] int32 (may be NULL with rotary_dim 0);  slots [tokens] int64, no slot twice
+ */
+int mi355_qk_norm_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                              const void* q_weight, const void* k_weight, int weight_dtype, const void* cos_table, const void* sin_table,
+                              int table_dtype, int64_t max_position, const int32_t* positions, const int64_t* slots, void* q_out,
+                              void* k_cache, void* v_cache, void* k_scale, void* v_scale, int tokens, int heads, int heads_kv, int dim,
+                              int rotary_dim, int interleaved, double eps, int page_size, int64_t n_phys_tokens, int x_dtype,
+                              int cache_dtype, void* hip_stream);
+
+/*
+ * Rows of a 4-bit cache as 16-bit values: k_out, v_out [tokens, heads_kv, dim] out_dtype (bf16: exact; fp16: rounded once), the rows of
+ * slots [tokens] int64; zeros for slots outside the pool.
+ */
+int mi355_kv_gather_fp4(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int64_t* slots,
+                        void* k_out, void* v_out, int tokens, int heads_kv, int dim, int page_size, int64_t n_phys_tokens, int out_dtype,
+                        void* hip_stream);
+
+/*
+ * mi355_gqa_paged_decode() over a 4-bit cache: one or more query tokens per sequence, arguments as there except
+ *   k, v           codes, k_scale, v_scale scale bytes in the layout above
+ *   page_size      a multiple of 16
+ *   max_pages      entries of a block-table row (<= bt_row_stride): lengths are clamped to max_pages * page_size
+ * A query row that sees no token (seqlens[b] == 0, or causal with q_len > seqlens[b]) is zeros.  Tokens that a row does not see
+ * do not change it, whatever their bytes are.  Both products accumulate in fp32; the query enters exactly (up to 2^-17 of the row's largest
+ * element), probabilities as bf16 (fp16 queries: as two bf16 parts).
+ * The query of the workspace's size touches no device; partial results are fp32.
+ */
+int mi355_gqa_paged_decode_fp4_workspace(int batch, int q_len, int heads, int heads_kv, int dim, int page_size, int q_dtype,
+                                         size_t* workspace_bytes);
+int mi355_gqa_paged_decode_fp4(const void* q, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale,
+                               const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride, int max_pages, void* out,
+                               void* workspace, size_t workspace_bytes, int batch, int q_len, int heads, int heads_kv, int dim,
+                               int page_size, int64_t n_phys_tokens, int q_dtype, float sm_scale, float softcap, int causal, void* hip_stream);
 
 #ifdef __cplusplus
 }

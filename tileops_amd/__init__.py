@@ -1,6 +1,6 @@
 """MI355X (gfx950) paged GQA decode attention behind the TileOPs operator contract.
 
-Public surface: the four ops, the backend seam, the manifest loader.  The HIP library is opened lazily on
+Public surface: the attention ops, the ops of a serving step around the cache, the backend seam, the manifest loader.  The HIP library is opened lazily on
 the first kernel build; importing this package touches no device.
 """
 
@@ -14,8 +14,20 @@ from .ops import (  # noqa: F401
     GroupedQueryAttentionMultiTokenDecodePagedWithKVCacheFwdOp,
     GroupedQueryAttentionPrefillPagedWithKVCacheFwdOp,
 )
+from .serving_ops import (  # noqa: F401
+    GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp,
+    PagedFP4KVCacheGatherFwdOp,
+    PagedKVCacheAllocFwdOp,
+    PagedKVCacheReleaseFwdOp,
+    QKNormRopePagedKVAppendFwdOp,
+)
 
 __all__ = [
+    "GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp",
+    "PagedFP4KVCacheGatherFwdOp",
+    "PagedKVCacheAllocFwdOp",
+    "PagedKVCacheReleaseFwdOp",
+    "QKNormRopePagedKVAppendFwdOp",
     "GroupedQueryAttentionDecodeWithKVCacheFwdOp",
     "GroupedQueryAttentionDecodePagedWithKVCacheFwdOp",
     "GroupedQueryAttentionMultiTokenDecodePagedWithKVCacheFwdOp",

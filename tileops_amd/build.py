@@ -19,7 +19,8 @@ LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libmi355_tileops.so"
 OBJ_DIR = PKG / "build"
 
-SOURCES = ["abi.hip", "paged_decode_generic.hip", "paged_decode_mfma.hip", "paged_cache_utils.hip"]
+SOURCES = ["abi.hip", "paged_decode_generic.hip", "paged_decode_mfma.hip", "paged_cache_utils.hip", "paged_cache_step.hip",
+           "paged_decode_fp4.hip"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_*_f32 out of scalar float code.
 HIPCC_FLAGS = [

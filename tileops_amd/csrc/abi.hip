@@ -686,4 +686,145 @@ int mi355_prefill_input_facts(const int32_t* cu_seqlens_q, const int32_t* cache_
   return MI355_OK;
 }
 
+int mi355_kv_alloc(const int32_t* cached, const int32_t* cu_seqlens_q, int32_t* block_table, int64_t bt_row_stride, int max_pages,
+                   const int32_t* free_pages, const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* seqlens_out,
+                   uint8_t* refused, int32_t* free_count_out, int batch, int total_q, int page_size, int n_pages, void* hip_stream) {
+  if (batch <= 0) return fail(MI355_EINVAL, "batch must be positive, got %d", batch);
+  if (total_q < 0 || total_q > INT_MAX - 4096) return fail(MI355_EINVAL, "total_q must be non-negative and below 2^31 - 4096, got %d", total_q);
+  if (page_size <= 0 || max_pages <= 0 || n_pages <= 0) return fail(MI355_EINVAL, "page_size, max_pages and n_pages must be positive");
+  if (bt_row_stride < max_pages) return fail(MI355_EINVAL, "bt_row_stride must be at least max_pages");
+  if (!cu_seqlens_q && total_q != batch) return fail(MI355_EINVAL, "without cu_seqlens_q every sequence has one token: total_q must be batch");
+  if (!cached || !block_table || !free_pages || !free_count || !seqlens_out || !refused || !free_count_out || (total_q > 0 && (!slots || !positions)))
+    return fail(MI355_EINVAL, "null pointer argument");
+  if (free_count_out == free_count) return fail(MI355_EINVAL, "free_count_out must not be free_count");
+  if (int rc = check_device()) return rc;
+  const char* err = launch_kv_alloc(cached, cu_seqlens_q, block_table, bt_row_stride, free_pages, free_count, slots, positions, seqlens_out,
+                                    refused, free_count_out, batch, total_q, page_size, max_pages, n_pages, (hipStream_t)hip_stream);
+  if (err) return fail(MI355_ELAUNCH, "kernel launch failed: %s", err);
+  return MI355_OK;
+}
+
+int mi355_kv_release(const uint8_t* finished, const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride, int max_pages,
+                     int32_t* free_pages, const int32_t* free_count, int32_t* seqlens_out, int32_t* free_count_out, int batch,
+                     int page_size, int n_pages, void* hip_stream) {
+  if (batch <= 0) return fail(MI355_EINVAL, "batch must be positive, got %d", batch);
+  if (page_size <= 0 || max_pages <= 0 || n_pages <= 0) return fail(MI355_EINVAL, "page_size, max_pages and n_pages must be positive");
+  if (bt_row_stride < max_pages) return fail(MI355_EINVAL, "bt_row_stride must be at least max_pages");
+  if (!finished || !seqlens || !block_table || !free_pages || !free_count || !seqlens_out || !free_count_out)
+    return fail(MI355_EINVAL, "null pointer argument");
+  if (free_count_out == free_count) return fail(MI355_EINVAL, "free_count_out must not be free_count");
+  if (int rc = check_device()) return rc;
+  const char* err = launch_kv_release(finished, seqlens, block_table, bt_row_stride, free_pages, free_count, seqlens_out, free_count_out, batch,
+                                      page_size, max_pages, n_pages, (hipStream_t)hip_stream);
+  if (err) return fail(MI355_ELAUNCH, "kernel launch failed: %s", err);
+  return MI355_OK;
+}
+
+int mi355_qk_norm_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                              const void* q_weight, const void* k_weight, int weight_dtype, const void* cos_table, const void* sin_table,
+                              int table_dtype, int64_t max_position, const int32_t* positions, const int64_t* slots, void* q_out,
+                              void* k_cache, void* v_cache, void* k_scale, void* v_scale, int tokens, int heads, int heads_kv, int dim,
+                              int rotary_dim, int interleaved, double eps, int page_size, int64_t n_phys_tokens, int x_dtype,
+                              int cache_dtype, void* hip_stream) {
+  if (tokens < 0) return fail(MI355_EINVAL, "tokens must be non-negative, got %d", tokens);
+  if (heads <= 0 || heads_kv <= 0) return fail(MI355_EINVAL, "heads and heads_kv must be positive");
+  if ((int64_t)heads + 2 * (int64_t)heads_kv > 65535) return fail(MI355_EUNSUPPORTED, "more than 65535 heads");
+  if (dim != 64 && dim != 128 && dim != 256) return fail(MI355_EUNSUPPORTED, "head dim %d is not served (64, 128 or 256)", dim);
+  if (!is_q_dtype(x_dtype)) return fail(MI355_EINVAL, "x_dtype must be bf16 or fp16, got code %d", x_dtype);
+  const bool fp8 = cache_dtype == MI355_DT_FP8_E4M3FN, fp4 = cache_dtype == MI355_DT_FP4_E2M1;
+  if (!fp8 && !fp4 && cache_dtype != x_dtype) return fail(MI355_EINVAL, "cache_dtype must be x_dtype, fp8_e4m3fn or fp4_e2m1, got code %d", cache_dtype);
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > dim) return fail(MI355_EINVAL, "rotary_dim must be even and in [0, dim], got %d", rotary_dim);
+  if (page_size <= 0) return fail(MI355_EINVAL, "page_size must be positive");
+  if (n_phys_tokens <= 0 || n_phys_tokens % page_size != 0) return fail(MI355_EINVAL, "n_phys_tokens must be a positive multiple of page_size");
+  if (n_phys_tokens > INT_MAX) return fail(MI355_EUNSUPPORTED, "the pool holds 2^31 or more tokens");
+  if (!(eps >= 0.0)) return fail(MI355_EINVAL, "eps must be non-negative");
+  if (rotary_dim > 0 && max_position <= 0) return fail(MI355_EINVAL, "max_position must be positive");
+  if ((q_weight || k_weight) && weight_dtype != x_dtype && weight_dtype != MI355_DT_FP32)
+    return fail(MI355_EINVAL, "weight_dtype must be x_dtype or fp32, got code %d", weight_dtype);
+  if (rotary_dim > 0 && table_dtype != x_dtype && table_dtype != MI355_DT_FP32)
+    return fail(MI355_EINVAL, "table_dtype must be x_dtype or fp32, got code %d", table_dtype);
+  if (tokens == 0) return MI355_OK;
+  if (!q || !k || !v || !slots || !q_out || !k_cache || !v_cache) return fail(MI355_EINVAL, "null pointer argument");
+  if (rotary_dim > 0 && (!cos_table || !sin_table || !positions)) return fail(MI355_EINVAL, "cos_table, sin_table and positions are required with rotary_dim > 0");
+  if ((fp8 || fp4) && (!k_scale || !v_scale)) return fail(MI355_EINVAL, "k_scale and v_scale are required with an fp8 or fp4 cache");
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 3) || ((q_stride | k_stride | v_stride) & 1))
+    return fail(MI355_EINVAL, "q, k and v must be 4-byte aligned with even token strides");
+  if (((uintptr_t)q_out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return fail(MI355_EINVAL, "q_out and the caches must be 16-byte aligned");
+  if (int rc = check_device()) return rc;
+  const char* err = launch_qk_norm_rope_append(q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, weight_dtype, cos_table, sin_table,
+                                               table_dtype, max_position, positions, slots, q_out, k_cache, v_cache, k_scale, v_scale, tokens,
+                                               heads, heads_kv, dim, rotary_dim, interleaved ? 1 : 0, eps, page_size, n_phys_tokens, x_dtype,
+                                               cache_dtype, (hipStream_t)hip_stream);
+  if (err) return fail(MI355_ELAUNCH, "kernel launch failed: %s", err);
+  return MI355_OK;
+}
+
+int mi355_kv_gather_fp4(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int64_t* slots,
+                        void* k_out, void* v_out, int tokens, int heads_kv, int dim, int page_size, int64_t n_phys_tokens, int out_dtype,
+                        void* hip_stream) {
+  if (tokens < 0) return fail(MI355_EINVAL, "tokens must be non-negative, got %d", tokens);
+  if (heads_kv <= 0 || heads_kv > 65535) return fail(MI355_EINVAL, "heads_kv must be in [1, 65535]");
+  if (dim != 64 && dim != 128 && dim != 256) return fail(MI355_EUNSUPPORTED, "head dim %d is not served (64, 128 or 256)", dim);
+  if (page_size <= 0) return fail(MI355_EINVAL, "page_size must be positive");
+  if (n_phys_tokens <= 0 || n_phys_tokens % page_size != 0) return fail(MI355_EINVAL, "n_phys_tokens must be a positive multiple of page_size");
+  if (!is_q_dtype(out_dtype)) return fail(MI355_EINVAL, "out_dtype must be bf16 or fp16, got code %d", out_dtype);
+  if ((int64_t)tokens * heads_kv * (dim / 8) / 256 >= INT_MAX) return fail(MI355_EUNSUPPORTED, "too many rows");
+  if (tokens == 0) return MI355_OK;
+  if (!k_codes || !v_codes || !k_scale || !v_scale || !slots || !k_out || !v_out) return fail(MI355_EINVAL, "null pointer argument");
+  if (((uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)k_codes | (uintptr_t)v_codes) & 15)
+    return fail(MI355_EINVAL, "codes and outputs must be 16-byte aligned");
+  if (int rc = check_device()) return rc;
+  const char* err = launch_kv_gather_fp4(k_codes, v_codes, k_scale, v_scale, slots, k_out, v_out, tokens, heads_kv, dim, page_size, n_phys_tokens,
+                                         out_dtype, (hipStream_t)hip_stream);
+  if (err) return fail(MI355_ELAUNCH, "kernel launch failed: %s", err);
+  return MI355_OK;
+}
+
+int mi355_gqa_paged_decode_fp4_workspace(int batch, int q_len, int heads, int heads_kv, int dim, int page_size, int q_dtype,
+                                         size_t* workspace_bytes) {
+  int rc = check_shape(batch, q_len, heads, heads_kv, dim, page_size, q_dtype, MI355_DT_FP8_E4M3FN);
+  if (rc) return rc;
+  if (page_size % 16 != 0) return fail(MI355_EUNSUPPORTED, "page_size %d is not served with an fp4 cache (a multiple of 16)", page_size);
+  if ((int64_t)q_len * heads > INT_MAX) return fail(MI355_EUNSUPPORTED, "q_len * heads exceeds 2^31 - 1");
+  const int rows = q_len * (heads / heads_kv);
+  if (workspace_bytes) *workspace_bytes = fp4_workspace_bytes(fp4_num_parts(heads_kv, rows, dim, kPlanCuCount), heads_kv, rows, dim);
+  return MI355_OK;
+}
+
+int mi355_gqa_paged_decode_fp4(const void* q, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale,
+                               const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride, int max_pages, void* out,
+                               void* workspace, size_t workspace_bytes, int batch, int q_len, int heads, int heads_kv, int dim,
+                               int page_size, int64_t n_phys_tokens, int q_dtype, float sm_scale, float softcap, int causal, void* hip_stream) {
+  int rc = mi355_gqa_paged_decode_fp4_workspace(batch, q_len, heads, heads_kv, dim, page_size, q_dtype, nullptr);
+  if (rc) return rc;
+  if (batch == 0) return MI355_OK;
+  if (!q || !k_codes || !v_codes || !k_scale || !v_scale || !seqlens || !block_table || !out)
+    return fail(MI355_EINVAL, "q, k, v, k_scale, v_scale, seqlens, block_table and out must be non-null");
+  if (n_phys_tokens <= 0 || n_phys_tokens % page_size != 0)
+    return fail(MI355_EINVAL, "n_phys_tokens (%lld) must be a positive multiple of page_size (%d)", (long long)n_phys_tokens, page_size);
+  if (n_phys_tokens / page_size > INT_MAX) return fail(MI355_EUNSUPPORTED, "the pool holds 2^31 or more pages");
+  if (max_pages <= 0 || bt_row_stride < max_pages) return fail(MI355_EINVAL, "max_pages must be positive and at most bt_row_stride");
+  if (!(softcap >= 0.f)) return fail(MI355_EINVAL, "softcap must be non-negative");
+  if (!(sm_scale == sm_scale)) return fail(MI355_EINVAL, "sm_scale is NaN");
+  if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)out) & 15)
+    return fail(MI355_EINVAL, "q, k, v, k_scale, v_scale and out must be 16-byte aligned");
+  const int64_t row_tokens = (int64_t)max_pages * page_size, max_len = row_tokens < INT_MAX ? row_tokens : INT_MAX;
+  if (fp4_max_units(batch, max_len) > INT_MAX)
+    return fail(MI355_EUNSUPPORTED, "block tables of %d x %d pages address more tokens than a call can count", batch, max_pages);
+  rc = check_device();
+  if (rc) return rc;
+  // (the partition count of this device, never more than what the workspace query plans for)
+  const int rows = q_len * (heads / heads_kv), cus = device_cu_count();
+  const int n_parts = fp4_num_parts(heads_kv, rows, dim, cus < kPlanCuCount ? cus : kPlanCuCount);
+  const size_t need = fp4_workspace_bytes(n_parts, heads_kv, rows, dim);
+  if (!workspace) return fail(MI355_EWORKSPACE, "workspace of %zu bytes required, got null", need);
+  if (workspace_bytes < need) return fail(MI355_EWORKSPACE, "workspace of %zu bytes required, got %zu", need, workspace_bytes);
+  if ((uintptr_t)workspace & 255) return fail(MI355_EWORKSPACE, "workspace must be 256-byte aligned");
+  const char* err = launch_decode_fp4(q, k_codes, v_codes, k_scale, v_scale, seqlens, block_table, bt_row_stride, (int)max_len, out, workspace, batch, q_len,
+                                      heads, heads_kv, dim, page_size, n_phys_tokens / page_size, q_dtype, sm_scale, softcap, causal ? 1 : 0,
+                                      n_parts, (hipStream_t)hip_stream);
+  if (err) return fail(MI355_ELAUNCH, "kernel launch failed: %s", err);
+  return MI355_OK;
+}
+
 }  // extern "C"

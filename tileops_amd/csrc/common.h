@@ -154,5 +154,28 @@ const char* launch_prefill_input_facts(const int32_t* cu_q, const int32_t* cache
 const char* launch_kv_append_fp8(const void* x_new, void* cache, float* scale, const int32_t* seqlens,
                                  const int32_t* block_table, int64_t bt_row_stride, int batch, int heads_kv, int dim,
                                  int page_size, int64_t n_pages, int x_dtype, hipStream_t s);
+// The cache side of a serving step (paged_cache_step.hip) and attention over a 4-bit cache (paged_decode_fp4.hip).
+const char* launch_kv_alloc(const int32_t* cached, const int32_t* cu_q, int32_t* block_table, int64_t bt_row_stride, const int32_t* free_pages,
+                            const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* seqlens_out, uint8_t* refused,
+                            int32_t* free_count_out, int batch, int total_q, int page_size, int max_pages, int n_pages, hipStream_t s);
+const char* launch_kv_release(const uint8_t* finished, const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride,
+                              int32_t* free_pages, const int32_t* free_count, int32_t* seqlens_out, int32_t* free_count_out, int batch,
+                              int page_size, int max_pages, int n_pages, hipStream_t s);
+const char* launch_qk_norm_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                       const void* q_weight, const void* k_weight, int weight_dtype, const void* cos_table,
+                                       const void* sin_table, int table_dtype, int64_t max_position, const int32_t* positions,
+                                       const int64_t* slots, void* q_out, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                                       int tokens, int heads, int heads_kv, int dim, int rotary_dim, int interleaved, double eps,
+                                       int page_size, int64_t n_phys_tokens, int x_dtype, int cache_dtype, hipStream_t s);
+const char* launch_kv_gather_fp4(const void* k, const void* v, const void* k_scale, const void* v_scale, const int64_t* slots, void* k_out,
+                                 void* v_out, int tokens, int heads_kv, int dim, int page_size, int64_t n_phys_tokens, int out_dtype,
+                                 hipStream_t s);
+int fp4_num_parts(int heads_kv, int rows, int dim, int compute_units);
+size_t fp4_workspace_bytes(int n_parts, int heads_kv, int rows, int dim);
+int64_t fp4_max_units(int64_t batch, int64_t max_len);
+const char* launch_decode_fp4(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, const int32_t* seqlens,
+                              const int32_t* block_table, int64_t bt_row_stride, int max_len, void* out, void* workspace, int batch,
+                              int q_len, int heads, int heads_kv, int dim, int page_size, int64_t n_pages, int q_dtype, float sm_scale, float softcap, int causal,
+                              int n_parts, hipStream_t s);
 
 }  // namespace mi355

@@ -104,4 +104,50 @@ __device__ __forceinline__ float to_logit2(float qk, float score_scale, float ca
 __device__ __forceinline__ float wave_xor_max(float x, int mask) { return fmaxf(x, __shfl_xor(x, mask, 64)); }
 __device__ __forceinline__ float wave_xor_sum(float x, int mask) { return x + __shfl_xor(x, mask, 64); }
 
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// Reductions over the four 16-lane groups of a wave (lanes c, c+16, c+32, c+48) with the gfx950 lane-swap
+// instructions: v_permlane16_swap exchanges odd 16-lane rows of its first operand with even rows of the
+// second, v_permlane32_swap exchanges the upper half of the first with the lower half of the second.  Fed the
+// same value twice they return (x of the even partner, x of the odd partner), so one max/add finishes a step
+// without touching the LDS crossbar.
+// Maxima as single instructions.  fmaxf() first quiets a possible signalling NaN in each operand whose origin
+// the compiler cannot see (one extra v_max per operand); the scores here are MFMA results or -inf.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float group_max(float x) {
+  u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = max2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// v_exp_f32: exp2 without the denormal-range fix-up of exp2f (arguments here are <= 0 or -inf; a result
+// below 2^-126 may flush to zero, which is what a softmax weight that small should be).
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Inclusive prefix sum over the 64 lanes on the data-parallel-primitive path (no LDS crossbar): four shifts inside each row
+// of 16 lanes, then lane 15 of rows 0 and 2 added to rows 1 and 3, then lane 31 to rows 2 and 3.
+__device__ __forceinline__ int wave_incl_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 }  // namespace mi355

@@ -1,0 +1,474 @@
+// The cache side of a serving step on gfx950: pages taken from and given back to a pool, the norm and rotation of query and
+// key rows with the append of keys and values, and the read-back of 4-bit rows.
+//
+// The 4-bit cache ("fp4" below): 32 consecutive head elements form a block of e2m1 codes (two to a byte, the lower nibble
+// first) with one power-of-two scale byte, x = code * 2^(byte - 127); byte 255 makes the block NaN.  Codes are
+// [n_pages, heads_kv, page_size, dim / 2], scales [n_pages, heads_kv, page_size, dim / 32]: the rows of one (page, kv head)
+// are contiguous, because a token-major pool would give every 64-byte row of a 128-byte line to another head's workgroup.
+#include <climits>
+
+#include "common.h"
+#include "device_utils.h"
+
+namespace mi355 {
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------- page allocation
+// Sums of page counts saturate at INT_MAX (both operands are in [0, INT_MAX], so the unsigned sum does not wrap): a sum
+// that saturates is more than any pool holds.
+__device__ __forceinline__ int sat_add(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)INT_MAX); }
+
+__device__ __forceinline__ int wave_sat_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x = sat_add(x, y);
+  }
+  return x;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int page_size) {  // tokens >= 0; the sum fits 32 unsigned bits
+  return (int)(((uint32_t)tokens + (uint32_t)page_size - 1u) / (uint32_t)page_size);
+}
+
+constexpr int kAllocThreads = 1024;
+
+// With c_b tokens cached and n_b to come, sequence b needs need_b = ceil((c_b + n_b) / page) - ceil(c_b / page) pages.  In batch
+// order, page i of the call is free_pages[free - 1 - i] (the list is a stack); b is served if its tokens fit its table row and
+// need_b is 0 or sum_{a <= b} need_a <= free.  A new page's first token lies in this call, so the thread of that token
+// writes the table entry, and token t's page is either an entry that this call leaves alone or a place in the list: no
+// workgroup waits for another.  Every workgroup sums the needs of the sequences up to its own tokens itself (a few loads: 1024
+// sequences a pass); the first one goes through all of them and writes what there is one of per sequence.
+//
+// Bound: the launch.  A decode step moves 2 KB, a prefill step 12 bytes a token.
+template <bool kChunks>  // false: one new token per sequence, token t is sequence t's
+__global__ __launch_bounds__(kAllocThreads) void kv_alloc_kernel(
+    const int32_t* __restrict__ cached, const int32_t* __restrict__ cu_q, int32_t* __restrict__ block_table, int64_t bt_row_stride,
+    const int32_t* __restrict__ free_pages, const int32_t* __restrict__ free_count, int64_t* __restrict__ slots,
+    int32_t* __restrict__ positions, int32_t* __restrict__ seqlens_out, uint8_t* __restrict__ refused,
+    int32_t* __restrict__ free_count_out, int batch, int total_q, int page_size, int max_pages, int n_pages) {
+  __shared__ int s_cu[kAllocThreads + 1], s_cached[kAllocThreads], s_first[kAllocThreads];
+  __shared__ int s_wave[kAllocThreads / 64];
+  __shared__ int s_taken;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int tok = blockIdx.x * kAllocThreads + t;  // (the launcher keeps total_q below 2^31 - 1024)
+  const int tok_end = min((int)(blockIdx.x + 1) * kAllocThreads, total_q);
+  const int free0 = min(max(free_count[0], 0), n_pages);
+  const int row_tokens = (int)min((int64_t)max_pages * page_size, (int64_t)INT_MAX);
+  int64_t slot = -1;
+  int pos = -1, carry = 0;
+  if (t == 0) s_taken = 0;
+  // the page of logical page lp of a served sequence whose first new page is number `first` of the call
+  auto place = [&](int b, int c, int first, int at) __attribute__((always_inline)) {
+    const int lp = at / page_size, off = at - lp * page_size, fresh = lp - pages_of(c, page_size);
+    int page;
+    if (fresh < 0) {
+      page = block_table[(int64_t)b * bt_row_stride + lp];
+    } else {
+      page = free_pages[free0 - 1 - (first + fresh)];  // 0 <= first + fresh < free0: the sequence is served
+      if (off == 0) block_table[(int64_t)b * bt_row_stride + lp] = page;
+    }
+    slot = (int64_t)page * page_size + off;
+    pos = at;
+  };
+  for (int base = 0; base < batch; base += kAllocThreads) {
+    const int nb = min(batch - base, kAllocThreads);
+    if (blockIdx.x != 0 && (kChunks ? cu_q[base] : base) >= tok_end) break;  // the same for the whole workgroup
+    const int b = base + t;
+    int q0 = 0, c = 0;
+    int64_t n = 0;
+    if (t < nb) {
+      q0 = kChunks ? cu_q[b] : b;
+      n = kChunks ? (int64_t)cu_q[b + 1] - q0 : 1;
+      c = cached[b];
+    }
+    const bool fits = n > 0 && c >= 0 && c + n <= row_tokens;
+    const int need = fits ? pages_of(c + (int)n, page_size) - pages_of(c, page_size) : 0;
+    int incl = wave_sat_scan(need);
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    int before = carry, total = carry;
+#pragma unroll
+    for (int w = 0; w < kAllocThreads / 64; w++) {
+      if (w < wave) before = sat_add(before, s_wave[w]);
+      total = sat_add(total, s_wave[w]);
+    }
+    incl = sat_add(before, incl);
+    const bool served = fits && (need == 0 || incl <= free0);
+    const int first = incl - need;
+    if (blockIdx.x == 0) {
+      if (t < nb) {
+        seqlens_out[b] = served ? c + (int)n : c;
+        refused[b] = n > 0 && !served;
+      }
+      if (served && need > 0) atomicMax(&s_taken, incl);
+    }
+    if constexpr (kChunks) {
+      s_cu[t] = q0;
+      if (t == nb - 1) s_cu[nb] = q0 + (int)max(n, (int64_t)0);
+      s_cached[t] = c;
+      s_first[t] = served ? first : -1;
+      __syncthreads();
+      if (tok < total_q && tok >= s_cu[0] && tok < s_cu[nb]) {
+        int lo = 0, hi = nb;  // the last sequence that starts at or before the token (empty ones start where the next does)
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_cu[mid] <= tok) lo = mid; else hi = mid;
+        }
+        const int64_t at = (int64_t)s_cached[lo] + (tok - s_cu[lo]);
+        if (s_first[lo] >= 0 && at < row_tokens) place(base + lo, s_cached[lo], s_first[lo], (int)at);
+      }
+      __syncthreads();  // the arrays are written again
+    } else {
+      if (b == tok && t < nb && served) place(b, c, first, c);
+      __syncthreads();
+    }
+    carry = total;
+  }
+  if (tok < total_q) {
+    slots[tok] = slot;
+    positions[tok] = pos;
+  }
+  if (blockIdx.x == 0) {
+    __syncthreads();
+    if (t == 0) free_count_out[0] = free0 - s_taken;
+  }
+}
+
+// Pages of finished sequences back onto the list: entry j of sequence b's row goes to place free + (pages of the finished
+// sequences before b) + j.  A workgroup of four waves takes four sequences, a wave each, and sums the pages of all sequences
+// before them itself.
+constexpr int kReleaseWaves = 4;
+__global__ __launch_bounds__(64 * kReleaseWaves) void kv_release_kernel(
+    const uint8_t* __restrict__ finished, const int32_t* __restrict__ seqlens, const int32_t* __restrict__ block_table,
+    int64_t bt_row_stride, int32_t* __restrict__ free_pages, const int32_t* __restrict__ free_count, int32_t* __restrict__ seqlens_out,
+    int32_t* __restrict__ free_count_out, int batch, int page_size, int max_pages, int n_pages) {
+  __shared__ int s_wave[kReleaseWaves], s_own[kReleaseWaves];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int b0 = blockIdx.x * kReleaseWaves;
+  const int free0 = min(max(free_count[0], 0), n_pages);
+  auto pages = [&](int b) { return finished[b] && seqlens[b] > 0 ? min(pages_of(seqlens[b], page_size), max_pages) : 0; };
+  int sum = 0;
+  for (int b = t; b < b0; b += 64 * kReleaseWaves) sum = sat_add(sum, pages(b));
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) sum = sat_add(sum, __shfl_xor(sum, m, 64));
+  const int b = b0 + wave, n = b < batch ? pages(b) : 0;
+  if (lane == 0) {
+    s_wave[wave] = sum;
+    s_own[wave] = n;
+    if (b < batch) seqlens_out[b] = finished[b] ? 0 : seqlens[b];
+  }
+  __syncthreads();
+  int first = free0, total = free0;
+#pragma unroll
+  for (int w = 0; w < kReleaseWaves; w++) {
+    first = sat_add(first, s_wave[w]);
+    total = sat_add(total, sat_add(s_wave[w], s_own[w]));
+    if (w < wave) first = sat_add(first, s_own[w]);
+  }
+  const int32_t* row = block_table + (int64_t)b * bt_row_stride;
+  const int fit = min(n, max(n_pages - first, 0));  // (never past the list, whatever the counts say)
+  for (int j = lane; j < fit; j += 64) free_pages[first + j] = row[j];
+  if (t == 0 && b0 + kReleaseWaves >= batch) free_count_out[0] = min(total, n_pages);
+}
+
+// ------------------------------------------------------------------------------------------------------- 4-bit blocks
+// Scale byte of a block from the largest magnitude's bit pattern: the smallest e >= -126 with amax <= 6 * 2^e, plus 127.
+// amax = m * 2^E with m in [1, 2), and 6 * 2^e = 1.5 * 2^(e + 2): e = E - 2 while m <= 1.5, else E - 1.  (As integers the
+// patterns of magnitudes order like the magnitudes, and infinities and NaN come out above all finite ones.)
+// e <= 126, and magnitudes are held to 3 * 2^126 first: a code of 4 would overflow 32 bits there.
+__device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255u;
+  const uint32_t bits = min(amax_bits, 0x7f400000u);  // 3 * 2^126
+  const int e = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x400000u ? 2 : 1);
+  return (uint32_t)(max(e, -126) + 127);
+}
+
+// Two elements -> one byte of codes (round to nearest, ties to the even code).  The scale is a power of two: dividing by it is exact.
+__device__ __forceinline__ uint32_t fp4_pack2(float a, float b, uint32_t scale_byte) {
+  const float lim = 0x1.8p127f;
+  a = fminf(fmaxf(a, -lim), lim);
+  b = fminf(fmaxf(b, -lim), lim);
+  const uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, __uint_as_float(scale_byte << 23), 0);
+  return scale_byte == 255u ? 0u : (w & 0xffu);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// ------------------------------------------------------------------------------- norm + rotation + append of new rows
+struct AppendParams {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;  // elements between tokens (heads are dim apart)
+  const void *q_weight, *k_weight;       // null: no norm
+  const void *cos_table, *sin_table;     // [max_position, rotary_dim / 2]
+  const int32_t* positions;
+  const int64_t* slots;
+  uint16_t* q_out;
+  void *k_cache, *v_cache, *k_scale, *v_scale;
+  int64_t n_tokens;  // of the pool
+  int tokens, heads, heads_kv, dim, rotary_dim, max_position, page_size;
+  double eps;
+  int weight_fp32, table_fp32, interleaved;
+};
+
+enum { kCache16 = 0, kCacheFp8 = 1, kCacheFp4 = 2 };
+
+template <typename XT>
+__device__ __forceinline__ float load_x(const uint16_t* p) {
+  uint32_t raw[1] = {*p};
+  float out[2];
+  Unpack<XT, 2>::run(raw, out);
+  return out[0];
+}
+template <typename XT>
+__device__ __forceinline__ float load_side(const void* p, int64_t i, int fp32) {
+  return fp32 ? ((const float*)p)[i] : load_x<XT>((const uint16_t*)p + i);
+}
+
+// One head of one token per wave, a pair of neighbouring elements per lane (two pairs at head dim 256).  R: the type that the
+// norm and the rotation are formed in.
+template <typename XT, typename R>
+__device__ __forceinline__ void norm_rotate_pair(const AppendParams& p, const uint16_t* x, const void* weight, int64_t tpos, int d, R rstd, float* out) {
+  auto normed = [&](int e) -> R {
+    const R v = (R)load_x<XT>(x + e);
+    return weight ? v * rstd * (R)load_side<XT>(weight, e, p.weight_fp32) : v;
+  };
+  const int half = p.rotary_dim >> 1;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int e = d + i;
+    R y = normed(e);
+    if (e < p.rotary_dim) {
+      const int f = p.interleaved ? e >> 1 : (e < half ? e : e - half);
+      const bool first = p.interleaved ? (e & 1) == 0 : e < half;
+      const R other = normed(p.interleaved ? e ^ 1 : (first ? e + half : e - half));
+      const R c = (R)load_side<XT>(p.cos_table, tpos * half + f, p.table_fp32), s = (R)load_side<XT>(p.sin_table, tpos * half + f, p.table_fp32);
+      y = first ? y * c - other * s : y * c + other * s;
+    }
+    out[i] = (float)y;
+  }
+}
+
+template <typename XT, typename R>
+__device__ __forceinline__ R head_rstd(const AppendParams& p, const uint16_t* x, const void* weight, int lane) {
+  if (!weight) return (R)1;
+  R sum = 0;
+  for (int d = 2 * lane; d < p.dim; d += 128) {
+    const R a = (R)load_x<XT>(x + d), b = (R)load_x<XT>(x + d + 1);
+    sum += a * a + b * b;
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m, 64);
+  return (R)1 / sqrt(sum / (R)p.dim + (R)p.eps);
+}
+
+template <typename XT, int CACHE>
+__global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 63;
+  const int unit = blockIdx.y * 4 + uni(threadIdx.x >> 6), t = blockIdx.x;
+  if (unit >= p.heads + 2 * p.heads_kv) return;
+  const bool is_q = unit < p.heads, is_k = !is_q && unit < p.heads + p.heads_kv;
+  const int h = is_q ? unit : is_k ? unit - p.heads : unit - p.heads - p.heads_kv;
+  const uint16_t* x = is_q ? p.q + t * p.q_stride : is_k ? p.k + t * p.k_stride : p.v + t * p.v_stride;
+  x += (int64_t)h * p.dim;
+  const int pos = p.rotary_dim ? p.positions[t] : 0;
+  const int64_t tpos = min(max(pos, 0), p.max_position - 1);  // never outside the tables
+  const int64_t slot = p.slots[t];
+  if (!is_q && (slot < 0 || slot >= p.n_tokens)) return;
+  const void* weight = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
+  float y[2][2];
+  const int pairs = p.dim >> 1;
+  // keys that become codes: in 64 bits, rounded to 32 once, so that a value next to a rounding border gets the same code
+  // whatever the order of a sum is
+  if (is_k && CACHE != kCache16) {
+    const double rstd = head_rstd<XT, double>(p, x, weight, lane);
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (lane + 64 * j < pairs) norm_rotate_pair<XT, double>(p, x, weight, tpos, 2 * (lane + 64 * j), rstd, y[j]);
+  } else {
+    const float rstd = head_rstd<XT, float>(p, x, weight, lane);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (lane + 64 * j >= pairs) continue;
+      if (is_q || is_k) {
+        norm_rotate_pair<XT, float>(p, x, weight, tpos, 2 * (lane + 64 * j), rstd, y[j]);
+      } else {
+        y[j][0] = load_x<XT>(x + 2 * (lane + 64 * j));
+        y[j][1] = load_x<XT>(x + 2 * (lane + 64 * j) + 1);
+      }
+    }
+  }
+  const int64_t token_row = slot * p.heads_kv + h;  // row of a token-major pool
+  if (is_q || CACHE == kCache16) {
+    uint16_t* dst = is_q ? p.q_out + ((int64_t)t * p.heads + h) * p.dim : (uint16_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int i = lane + 64 * j;
+      if (i < pairs) ((uint32_t*)dst)[i] = (uint32_t)f32_to_elem_bits<XT>(y[j][0]) | ((uint32_t)f32_to_elem_bits<XT>(y[j][1]) << 16);
+    }
+    return;
+  }
+  if (CACHE == kCacheFp8) {
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (lane + 64 * j < pairs) amax = fmaxf(amax, fmaxf(fabsf(y[j][0]), fabsf(y[j][1])));
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
+    const float sc = fmaxf(amax, 1e-4f) / 448.0f;
+    if (lane == 0) ((float*)(is_k ? p.k_scale : p.v_scale))[token_row] = sc;
+    uint8_t* dst = (uint8_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int i = lane + 64 * j;
+      if (i >= pairs) continue;
+      const float a = fminf(fmaxf(y[j][0] / sc, -448.0f), 448.0f), b = fminf(fmaxf(y[j][1] / sc, -448.0f), 448.0f);
+      ((uint16_t*)dst)[i] = (uint16_t)(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0u, false) & 0xffff);
+    }
+    return;
+  }
+  // fp4: sixteen lanes hold a block
+  const int64_t page = slot / p.page_size;
+  const int64_t row = (page * p.heads_kv + h) * p.page_size + (slot - page * p.page_size);
+  uint8_t* codes = (uint8_t*)(is_k ? p.k_cache : p.v_cache) + row * (p.dim >> 1);
+  uint8_t* scales = (uint8_t*)(is_k ? p.k_scale : p.v_scale) + row * (p.dim >> 5);
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int i = lane + 64 * j;
+    if (i >= pairs) continue;  // (whole groups of sixteen lanes: dim is a multiple of 32)
+    uint32_t amax = max(abs_bits(y[j][0]), abs_bits(y[j][1]));
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, m, 64));
+    const uint32_t byte = fp4_scale_byte(amax);
+    codes[i] = (uint8_t)fp4_pack2(y[j][0], y[j][1], byte);
+    if ((lane & 15) == 0) scales[i >> 4] = (uint8_t)byte;
+  }
+}
+
+// --------------------------------------------------------------------------------------------- rows of the 4-bit cache
+// Eight elements per thread (four bytes of codes in, sixteen out).  Slots outside the pool give zeros.
+template <typename XT>
+__global__ __launch_bounds__(256) void kv_gather_fp4_kernel(const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
+                                                            const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
+                                                            const int64_t* __restrict__ slots, uint4* __restrict__ k_out,
+                                                            uint4* __restrict__ v_out, int tokens, int heads_kv, int dim, int page_size,
+                                                            int64_t n_tokens) {
+  const int per_row = dim >> 3, per_token = heads_kv * per_row;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)tokens * per_token) return;
+  const int t = (int)(i / per_token), e = (int)(i - (int64_t)t * per_token), h = e / per_row, c = e - h * per_row;
+  const int64_t slot = slots[t];
+  uint4 r = {0, 0, 0, 0};
+  if (slot >= 0 && slot < n_tokens) {
+    const int64_t page = slot / page_size, row = (page * heads_kv + h) * page_size + (slot - page * page_size);
+    const uint32_t w = *(const uint32_t*)((blockIdx.y ? v : k) + row * (dim >> 1) + 4 * c);
+    const float sc = __uint_as_float((uint32_t)(blockIdx.y ? v_scale : k_scale)[row * (dim >> 5) + (c >> 2)] << 23);
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+    if constexpr (__is_same(XT, bf16_tag)) {
+      r.x = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+      r.y = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+      r.z = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+      r.w = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+    } else {
+      r.x = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0));
+      r.y = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1));
+      r.z = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2));
+      r.w = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3));
+    }
+  }
+  (blockIdx.y ? v_out : k_out)[i] = r;
+}
+
+const char* launched() {
+  hipError_t e = hipGetLastError();
+  return e == hipSuccess ? nullptr : hipGetErrorString(e);
+}
+
+}  // namespace
+
+const char* launch_kv_alloc(const int32_t* cached, const int32_t* cu_q, int32_t* block_table, int64_t bt_row_stride, const int32_t* free_pages,
+                            const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* seqlens_out, uint8_t* refused,
+                            int32_t* free_count_out, int batch, int total_q, int page_size, int max_pages, int n_pages, hipStream_t s) {
+  const dim3 grid(total_q > 0 ? (total_q + kAllocThreads - 1) / kAllocThreads : 1), block(kAllocThreads);
+  if (cu_q)
+    hipLaunchKernelGGL(kv_alloc_kernel<true>, grid, block, 0, s, cached, cu_q, block_table, bt_row_stride, free_pages, free_count, slots,
+                       positions, seqlens_out, refused, free_count_out, batch, total_q, page_size, max_pages, n_pages);
+  else
+    hipLaunchKernelGGL(kv_alloc_kernel<false>, grid, block, 0, s, cached, cu_q, block_table, bt_row_stride, free_pages, free_count, slots,
+                       positions, seqlens_out, refused, free_count_out, batch, total_q, page_size, max_pages, n_pages);
+  return launched();
+}
+
+const char* launch_kv_release(const uint8_t* finished, const int32_t* seqlens, const int32_t* block_table, int64_t bt_row_stride,
+                              int32_t* free_pages, const int32_t* free_count, int32_t* seqlens_out, int32_t* free_count_out, int batch,
+                              int page_size, int max_pages, int n_pages, hipStream_t s) {
+  hipLaunchKernelGGL(kv_release_kernel, dim3((batch + kReleaseWaves - 1) / kReleaseWaves), dim3(64 * kReleaseWaves), 0, s, finished, seqlens,
+                     block_table, bt_row_stride, free_pages, free_count, seqlens_out, free_count_out, batch, page_size, max_pages, n_pages);
+  return launched();
+}
+
+const char* launch_qk_norm_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                       const void* q_weight, const void* k_weight, int weight_dtype, const void* cos_table,
+                                       const void* sin_table, int table_dtype, int64_t max_position, const int32_t* positions,
+                                       const int64_t* slots, void* q_out, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                                       int tokens, int heads, int heads_kv, int dim, int rotary_dim, int interleaved, double eps,
+                                       int page_size, int64_t n_phys_tokens, int x_dtype, int cache_dtype, hipStream_t s) {
+  AppendParams p;
+  p.q = (const uint16_t*)q;
+  p.k = (const uint16_t*)k;
+  p.v = (const uint16_t*)v;
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.cos_table = cos_table;
+  p.sin_table = sin_table;
+  p.positions = positions;
+  p.slots = slots;
+  p.q_out = (uint16_t*)q_out;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.n_tokens = n_phys_tokens;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.heads_kv = heads_kv;
+  p.dim = dim;
+  p.rotary_dim = rotary_dim;
+  p.max_position = (int)(max_position < INT_MAX ? max_position : INT_MAX);
+  p.page_size = page_size;
+  p.eps = eps;
+  p.weight_fp32 = weight_dtype == MI355_DT_FP32;
+  p.table_fp32 = table_dtype == MI355_DT_FP32;
+  p.interleaved = interleaved;
+  const int cache = cache_dtype == MI355_DT_FP4_E2M1 ? kCacheFp4 : cache_dtype == MI355_DT_FP8_E4M3FN ? kCacheFp8 : kCache16;
+  const dim3 grid(tokens, (heads + 2 * heads_kv + 3) / 4), block(256);
+#define MI355_LAUNCH_APPEND(XT)                                                                                      \
+  do {                                                                                                               \
+    if (cache == kCacheFp4) hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCacheFp4>), grid, block, 0, s, p);   \
+    else if (cache == kCacheFp8) hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCacheFp8>), grid, block, 0, s, p); \
+    else hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCache16>), grid, block, 0, s, p);                       \
+  } while (0)
+  if (x_dtype == MI355_DT_BF16) MI355_LAUNCH_APPEND(bf16_tag);
+  else MI355_LAUNCH_APPEND(fp16_tag);
+#undef MI355_LAUNCH_APPEND
+  return launched();
+}
+
+const char* launch_kv_gather_fp4(const void* k, const void* v, const void* k_scale, const void* v_scale, const int64_t* slots, void* k_out,
+                                 void* v_out, int tokens, int heads_kv, int dim, int page_size, int64_t n_phys_tokens, int out_dtype,
+                                 hipStream_t s) {
+  const int64_t items = (int64_t)tokens * heads_kv * (dim / 8);
+  const dim3 grid((unsigned)((items + 255) / 256), 2), block(256);
+  auto kern = out_dtype == MI355_DT_BF16 ? kv_gather_fp4_kernel<bf16_tag> : kv_gather_fp4_kernel<fp16_tag>;
+  hipLaunchKernelGGL(kern, grid, block, 0, s, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, slots,
+                     (uint4*)k_out, (uint4*)v_out, tokens, heads_kv, dim, page_size, n_phys_tokens);
+  return launched();
+}
+
+}  // namespace mi355

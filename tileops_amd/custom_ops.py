@@ -10,10 +10,16 @@ kernel class's ``forward`` goes through one of the operators below.  Each operat
 * allocates the output and the workspace with torch inside its implementation and enqueues the HIP kernels on
   the current stream (nothing else: no host read-back, no synchronisation),
 * has a fake implementation that only states the output's shape and dtype (``empty_like(q)``),
-* declares the page pools it appends to as mutated (the two prefill operators).
+* declares the page pools it appends to as mutated (the two prefill operators, the append), and likewise the block table
+  and the list of free pages that the page operators write.
 
 Operator names: ``tileops_amd::gqa_paged_decode``, ``tileops_amd::gqa_decode``, ``tileops_amd::gqa_prefill_paged``,
-``tileops_amd::gqa_prefill_paged_rope``.
+``tileops_amd::gqa_prefill_paged_rope``, and of a serving step around a paged cache ``tileops_amd::kv_alloc``, ``tileops_amd::kv_release``,
+``tileops_amd::qk_norm_rope_append``, ``tileops_amd::kv_gather_fp4``, ``tileops_amd::gqa_paged_decode_fp4``.
+
+An operator call through torch's dispatcher costs the host about 30 us, several times what the kernels of a decode step's
+bookkeeping run.  The serving-step kernel classes therefore call the implementations below (``*_impl``) directly where the dispatcher
+has nothing to add -- plain tensors outside any tracing, see ``plain_call``.
 """
 
 from __future__ import annotations
@@ -24,10 +30,12 @@ import torch
 
 from . import native
 
-__all__ = ["OP_NAMES", "gqa_decode", "gqa_paged_decode", "gqa_prefill_paged", "gqa_prefill_paged_rope"]
+__all__ = ["OP_NAMES", "gqa_decode", "gqa_paged_decode", "gqa_paged_decode_fp4", "gqa_prefill_paged", "gqa_prefill_paged_rope", "kv_alloc",
+           "kv_gather_fp4", "kv_release", "plain_call", "qk_norm_rope_append"]
 
 OP_NAMES = ("tileops_amd::gqa_paged_decode", "tileops_amd::gqa_decode", "tileops_amd::gqa_prefill_paged",
-            "tileops_amd::gqa_prefill_paged_rope")
+            "tileops_amd::gqa_prefill_paged_rope", "tileops_amd::kv_alloc", "tileops_amd::kv_release", "tileops_amd::qk_norm_rope_append",
+            "tileops_amd::kv_gather_fp4", "tileops_amd::gqa_paged_decode_fp4")
 
 # (workspace bytes, partition count) per shape: a workspace query touches no device and never changes its answer
 _decode_plans: dict[tuple, tuple[int, int]] = {}
@@ -142,4 +150,131 @@ def gqa_prefill_paged_rope(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
 @gqa_prefill_paged_rope.register_fake
 def _(q, k_new, v_new, k_pages, v_pages, cos_table, sin_table, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q, heads,
       heads_kv, dim, page_size, rotary_dim, sm_scale, softcap, causal, kernel):
+    return torch.empty_like(q)
+
+
+# --- a serving step around a paged cache ------------------------------------------------------------------------------------
+def plain_call(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on *tensors* needs nothing of torch's dispatcher: no tracing, no dispatch mode, no tensor subclass, no gradient."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or (grad and t.requires_grad)):
+            return False
+    return True
+
+
+def kv_alloc_impl(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  cu_seqlens_q: Optional[torch.Tensor], total_q: int, page_size: int
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages and slots of a step's new tokens (``mi355_kv_alloc``); writes the new entries of ``block_table``."""
+    native.require_gfx950(block_table.device)
+    outs = _kv_alloc_outputs(cache_seqlens, total_q)
+    native.kv_alloc(cache_seqlens, cu_seqlens_q, block_table, free_pages, free_count, *outs, max_pages=block_table.shape[1], page_size=page_size)
+    return outs
+
+
+def _kv_alloc_outputs(cache_seqlens, total_q):
+    device, batch = cache_seqlens.device, cache_seqlens.shape[0]
+    return (torch.empty(total_q, dtype=torch.int64, device=device), torch.empty(total_q, dtype=torch.int32, device=device),
+            torch.empty(batch, dtype=torch.int32, device=device), torch.empty(batch, dtype=torch.bool, device=device),
+            torch.empty(1, dtype=torch.int32, device=device))
+
+
+kv_alloc = torch.library.custom_op("tileops_amd::kv_alloc", kv_alloc_impl, mutates_args=("block_table",))
+
+
+@kv_alloc.register_fake
+def _(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q, page_size):
+    return _kv_alloc_outputs(cache_seqlens, total_q)
+
+
+def kv_release_impl(finished: torch.Tensor, seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                    page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pages of finished sequences back onto the list (``mi355_kv_release``); writes ``free_pages`` behind its free ones."""
+    native.require_gfx950(block_table.device)
+    outs = (torch.empty_like(seqlens), torch.empty_like(free_count))
+    native.kv_release(finished, seqlens, block_table, free_pages, free_count, *outs, max_pages=block_table.shape[1], page_size=page_size)
+    return outs
+
+
+kv_release = torch.library.custom_op("tileops_amd::kv_release", kv_release_impl, mutates_args=("free_pages",))
+
+
+@kv_release.register_fake
+def _(finished, seqlens, block_table, free_pages, free_count, page_size):
+    return torch.empty_like(seqlens), torch.empty_like(free_count)
+
+
+def qk_norm_rope_append_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                             cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                             slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor],
+                             v_scale: Optional[torch.Tensor], rotary_dim: int, interleaved: bool, eps: float, page_size: int,
+                             cache_code: int) -> torch.Tensor:
+    """Norm + rotation of query and key rows, append of keys and values (``mi355_qk_norm_rope_append``)."""
+    native.require_gfx950(q.device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    native.qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, out, k_cache, v_cache, k_scale, v_scale,
+                               rotary_dim=rotary_dim, interleaved=interleaved, eps=eps, page_size=page_size, cache_dtype=cache_code)
+    return out
+
+
+qk_norm_rope_append = torch.library.custom_op("tileops_amd::qk_norm_rope_append", qk_norm_rope_append_impl,
+                                              mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+
+
+@qk_norm_rope_append.register_fake
+def _(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, rotary_dim, interleaved,
+      eps, page_size, cache_code):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def kv_gather_fp4_impl(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
+                       dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of a 4-bit cache as 16-bit values (``mi355_kv_gather_fp4``)."""
+    native.require_gfx950(k.device)
+    outs = _kv_gather_outputs(k, slot_mapping, dtype)
+    native.kv_gather_fp4(k, v, k_scale, v_scale, slot_mapping, *outs, page_size=k.shape[2])
+    return outs
+
+
+def _kv_gather_outputs(k, slot_mapping, dtype):
+    shape = (slot_mapping.shape[0], k.shape[1], 2 * k.shape[3])
+    return torch.empty(shape, dtype=dtype, device=k.device), torch.empty(shape, dtype=dtype, device=k.device)
+
+
+kv_gather_fp4 = torch.library.custom_op("tileops_amd::kv_gather_fp4", kv_gather_fp4_impl, mutates_args=())
+
+
+@kv_gather_fp4.register_fake
+def _(k, v, k_scale, v_scale, slot_mapping, dtype):
+    return _kv_gather_outputs(k, slot_mapping, dtype)
+
+
+_decode_fp4_plans: dict[tuple, int] = {}
+
+
+def gqa_paged_decode_fp4_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                              real_seqlen_kv: torch.Tensor, block_table: torch.Tensor, q_len: int, heads: int, heads_kv: int, dim: int,
+                              page_size: int, sm_scale: float, softcap: float, causal: bool) -> torch.Tensor:
+    """Paged GQA decode over a 4-bit cache (``mi355_gqa_paged_decode_fp4``)."""
+    native.require_gfx950(q.device)
+    batch = q.shape[0]
+    key = (batch, q_len, heads, heads_kv, dim, page_size, q.dtype)
+    nbytes = _decode_fp4_plans.get(key)
+    if nbytes is None:
+        nbytes = _decode_fp4_plans[key] = native.decode_fp4_workspace(*key)
+    out = torch.empty_like(q)
+    native.paged_decode_fp4(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table, out, torch.empty(nbytes, dtype=torch.uint8, device=q.device),
+                            q_len=q_len, heads=heads, heads_kv=heads_kv, dim=dim, page_size=page_size, sm_scale=sm_scale, softcap=softcap,
+                            causal=causal)
+    return out
+
+
+gqa_paged_decode_fp4 = torch.library.custom_op("tileops_amd::gqa_paged_decode_fp4", gqa_paged_decode_fp4_impl, mutates_args=())
+
+
+@gqa_paged_decode_fp4.register_fake
+def _(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table, q_len, heads, heads_kv, dim, page_size, sm_scale, softcap, causal):
     return torch.empty_like(q)

@@ -17,7 +17,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmi355_tileops.so"
 ABI_VERSION = 1
 
-DT_BF16, DT_FP16, DT_FP8_E4M3FN = 0, 1, 2
+DT_BF16, DT_FP16, DT_FP8_E4M3FN, DT_FP32, DT_FP4_E2M1 = 0, 1, 2, 3, 4
 KERNEL_AUTO, KERNEL_GENERIC, KERNEL_MFMA = 0, 1, 2
 KERNEL_FLAG_SKIP_COMBINE = 0x100  # this package's benchmark only (csrc/common.h): attention kernel alone, partials left unmerged
 KERNEL_NAMES = {KERNEL_AUTO: "auto", KERNEL_GENERIC: "generic", KERNEL_MFMA: "mfma"}
@@ -37,6 +37,12 @@ EXPORTED_SYMBOLS = (
     "mi355_gather_probe",
     "mi355_kv_append_fp8",
     "mi355_prefill_input_facts",
+    "mi355_kv_alloc",
+    "mi355_kv_release",
+    "mi355_qk_norm_rope_append",
+    "mi355_kv_gather_fp4",
+    "mi355_gqa_paged_decode_fp4_workspace",
+    "mi355_gqa_paged_decode_fp4",
 )
 
 
@@ -111,6 +117,26 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mi355_kv_append_fp8.restype = _c_int
     lib.mi355_kv_append_fp8.argtypes = [
         _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_vp,
+    ]
+    lib.mi355_kv_alloc.restype = _c_int
+    lib.mi355_kv_alloc.argtypes = [
+        _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp,
+    ]
+    lib.mi355_kv_release.restype = _c_int
+    lib.mi355_kv_release.argtypes = [_c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp]
+    lib.mi355_qk_norm_rope_append.restype = _c_int
+    lib.mi355_qk_norm_rope_append.argtypes = [
+        _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_int, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
+        _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_double, _c_int, _c_i64, _c_int, _c_int, _c_vp,
+    ]
+    lib.mi355_kv_gather_fp4.restype = _c_int
+    lib.mi355_kv_gather_fp4.argtypes = [_c_vp] * 7 + [_c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_vp]
+    lib.mi355_gqa_paged_decode_fp4_workspace.restype = _c_int
+    lib.mi355_gqa_paged_decode_fp4_workspace.argtypes = [_c_int] * 7 + [ctypes.POINTER(_c_sz)]
+    lib.mi355_gqa_paged_decode_fp4.restype = _c_int
+    lib.mi355_gqa_paged_decode_fp4.argtypes = [
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_sz, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_i64, _c_int, _c_f32, _c_f32, _c_int, _c_vp,
     ]
 
 
@@ -387,3 +413,84 @@ def prefill_input_facts(cu_seqlens_q: torch.Tensor, cache_seqlens: torch.Tensor,
         cache_seqlens.shape[0], block_table.shape[1], facts.data_ptr(), stream.cuda_stream))
     stream.synchronize()
     return facts.tolist()
+
+
+def _on_device(fn, tensor: torch.Tensor, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of *tensor*'s device, which is made current for the call if it is not."""
+    index = tensor.device.index
+    if index == torch.cuda.current_device():
+        _check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        return
+    with torch.cuda.device(index):
+        _check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _row_stride(block_table: torch.Tensor) -> int:
+    # (a table of one row may carry any stride: it says nothing)
+    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def kv_alloc(cached: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor], block_table: torch.Tensor, free_pages: torch.Tensor,
+             free_count: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, seqlens_out: torch.Tensor, refused: torch.Tensor,
+             free_count_out: torch.Tensor, *, max_pages: int, page_size: int) -> None:
+    """Enqueue the page allocation of one step (``mi355_kv_alloc``).  Arguments are assumed validated."""
+    _on_device(load().mi355_kv_alloc, block_table, cached.data_ptr(), _ptr(cu_seqlens_q), block_table.data_ptr(), _row_stride(block_table), max_pages,
+               free_pages.data_ptr(), free_count.data_ptr(), slots.data_ptr(), positions.data_ptr(), seqlens_out.data_ptr(), refused.data_ptr(),
+               free_count_out.data_ptr(), cached.shape[0], slots.shape[0], page_size, free_pages.shape[0])
+
+
+def kv_release(finished: torch.Tensor, seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+               seqlens_out: torch.Tensor, free_count_out: torch.Tensor, *, max_pages: int, page_size: int) -> None:
+    """Enqueue the return of finished sequences' pages (``mi355_kv_release``)."""
+    _on_device(load().mi355_kv_release, block_table, finished.data_ptr(), seqlens.data_ptr(), block_table.data_ptr(), _row_stride(block_table),
+               max_pages, free_pages.data_ptr(), free_count.data_ptr(), seqlens_out.data_ptr(), free_count_out.data_ptr(), seqlens.shape[0],
+               page_size, free_pages.shape[0])
+
+
+_SIDE_DTYPES = {torch.bfloat16: DT_BF16, torch.float16: DT_FP16, torch.float32: DT_FP32}
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                        cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                        slots: torch.Tensor, q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], *, rotary_dim: int, interleaved: bool, eps: float,
+                        page_size: int, cache_dtype: int) -> None:
+    """Enqueue norm + rotation + append of a step's rows (``mi355_qk_norm_rope_append``); ``cache_dtype`` is a ``DT_`` code."""
+    tokens, heads, dim = q.shape
+    weight = q_weight if q_weight is not None else k_weight
+    x_dtype = dtype_code(q.dtype)
+    pool = k_cache.shape[0] * page_size if cache_dtype == DT_FP4_E2M1 else k_cache.shape[0]
+    _on_device(load().mi355_qk_norm_rope_append, q, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+               _ptr(q_weight), _ptr(k_weight), x_dtype if weight is None else _SIDE_DTYPES[weight.dtype], _ptr(cos_table), _ptr(sin_table),
+               x_dtype if cos_table is None else _SIDE_DTYPES[cos_table.dtype], 0 if cos_table is None else cos_table.shape[0], _ptr(positions),
+               slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), tokens, heads, k.shape[1],
+               dim, rotary_dim, int(interleaved), eps, page_size, pool, x_dtype, cache_dtype)
+
+
+def kv_gather_fp4(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor,
+                  v_out: torch.Tensor, *, page_size: int) -> None:
+    """Enqueue the read-back of 4-bit rows (``mi355_kv_gather_fp4``)."""
+    tokens, heads_kv, dim = k_out.shape
+    _on_device(load().mi355_kv_gather_fp4, k, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), k_out.data_ptr(),
+               v_out.data_ptr(), tokens, heads_kv, dim, page_size, k.shape[0] * page_size, dtype_code(k_out.dtype))
+
+
+def decode_fp4_workspace(batch: int, q_len: int, heads: int, heads_kv: int, dim: int, page_size: int, q_dtype: torch.dtype) -> int:
+    """Workspace bytes of a decode call over a 4-bit cache.  Touches no device."""
+    nbytes = _c_sz(0)
+    _check(load().mi355_gqa_paged_decode_fp4_workspace(batch, q_len, heads, heads_kv, dim, page_size, dtype_code(q_dtype), ctypes.byref(nbytes)))
+    return int(nbytes.value)
+
+
+def paged_decode_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, seqlens: torch.Tensor,
+                     block_table: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor, *, q_len: int, heads: int, heads_kv: int, dim: int,
+                     page_size: int, sm_scale: float, softcap: float, causal: bool) -> None:
+    """Enqueue one decode call over a 4-bit cache (``mi355_gqa_paged_decode_fp4``).  Arguments are assumed validated."""
+    _on_device(load().mi355_gqa_paged_decode_fp4, q, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+               seqlens.data_ptr(), block_table.data_ptr(), _row_stride(block_table), block_table.shape[1], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+               seqlens.shape[0], q_len, heads, heads_kv, dim, page_size, k.shape[0] * page_size, dtype_code(q.dtype), sm_scale, softcap,
+               int(causal))

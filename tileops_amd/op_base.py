@@ -25,7 +25,7 @@ _UNRESOLVED = object()
 
 _DTYPES = {
     "float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32, "int32": torch.int32,
-    "int64": torch.int64, "float8_e4m3fn": torch.float8_e4m3fn,
+    "int64": torch.int64, "float8_e4m3fn": torch.float8_e4m3fn, "uint8": torch.uint8, "bool": torch.bool,
 }
 
 

@@ -98,6 +98,31 @@ def gqa_decode_roofline(op: Optional[Any] = None, **kwargs: Any) -> tuple[int, i
     return algorithmic_flops(sum_len=seen["sum_len"], q_len=1, heads=heads, dim=dim), b["total"] - 4 * batch
 
 
+def gqa_decode_paged_fp4_roofline(op: Optional[Any] = None, **kwargs: Any) -> tuple[int, int]:
+    """Paged GQA decode over a 4-bit cache: as ``gqa_decode_paged_roofline``, with ``dim / 2`` bytes of codes and ``dim / 32`` of scales per
+    K and V row; the pool priced once until the op has seen a call (``observe_call``)."""
+    d = _fields(op, kwargs)
+    q_len = 1
+    if "q_shape" in d:
+        qs = tuple(d["q_shape"])
+        if len(qs) == 4:
+            batch, q_len, heads, dim = qs
+        else:
+            batch, heads, dim = qs
+        seqlen_kv, heads_kv, _ = d["kv_shape"]
+    else:
+        batch, heads, heads_kv, seqlen_kv, dim = d["batch"], d["heads"], d["heads_kv"], d["seqlen_kv"], d["dim"]
+        q_len = int(d.get("q_len", 1) or 1)
+    seen = d.get("_seen_call")
+    row = dim // 2 + dim // 32
+    qo, lens = 2 * batch * q_len * heads * dim * 2, 4 * batch
+    if seen is None:
+        pages = (seqlen_kv + int(d["page_size"]) - 1) // int(d["page_size"])
+        return int(4 * batch * q_len * heads * seqlen_kv * dim), int(2 * seqlen_kv * heads_kv * row + qo + lens + 4 * batch * pages)
+    return (algorithmic_flops(sum_len=seen["sum_len"], q_len=q_len, heads=heads, dim=dim),
+            2 * seen["sum_len"] * heads_kv * row + qo + lens + 4 * seen["sum_pages"])
+
+
 def _distribute_total(total: int, batch: int, max_len: int) -> list[int]:
     """src/tileops/perf/formulas.py:467-475."""
     lengths, remaining = [0] * batch, total

@@ -803,6 +803,7 @@ int mi355_gqa_paged_decode_fp4(const void* q, const void* k_codes, const void* v
   if (n_phys_tokens <= 0 || n_phys_tokens % page_size != 0)
     return fail(MI355_EINVAL, "n_phys_tokens (%lld) must be a positive multiple of page_size (%d)", (long long)n_phys_tokens, page_size);
   if (n_phys_tokens / page_size > INT_MAX) return fail(MI355_EUNSUPPORTED, "the pool holds 2^31 or more pages");
+  if ((int64_t)heads_kv * page_size * (dim / 2) > INT_MAX) return fail(MI355_EUNSUPPORTED, "a page of codes holds 2^31 or more bytes");
   if (max_pages <= 0 || bt_row_stride < max_pages) return fail(MI355_EINVAL, "max_pages must be positive and at most bt_row_stride");
   if (!(softcap >= 0.f)) return fail(MI355_EINVAL, "softcap must be non-negative");
   if (!(sm_scale == sm_scale)) return fail(MI355_EINVAL, "sm_scale is NaN");

@@ -15,8 +15,9 @@
 //  * PV: O^T += V^T.P^T on v_mfma_f32_16x16x32_bf16.  Lane (c, g) loads the head elements [c * D/16, (c + 1) * D/16) of its eight
 //    tokens -- those whose probabilities it holds already -- widens them with their scale (v_cvt_scalef32_pk_bf16_fp4) and pairs the
 //    tokens with byte permutes: V needs no LDS, P does not move.
-//  * K, V and scales go from memory to registers a tile ahead of their use.
+//  * K, V and scales go from memory to registers, a tile ahead of their use, across the borders of sequences.
 #include <climits>
+#include <type_traits>
 
 #include "common.h"
 #include "device_utils.h"
@@ -42,7 +43,7 @@ struct Fp4Params {
   int64_t bt_row_stride;
   uint16_t* out;
   float *part_o, *part_lse;
-  int batch, q_len, heads, heads_kv, page_size, group, rows, row_groups, n_parts, max_len, causal;
+  int batch, q_len, heads, heads_kv, page_size, group, rows, row_groups, n_parts, max_len, causal, negate_q;
   int n_pages;
   float score_scale, cap_log2e, inv_cap_scale;
 };
@@ -50,33 +51,34 @@ struct Fp4Params {
 __device__ __forceinline__ int len_of(const Fp4Params& p, int b) { return min(max(p.seqlens[b], 0), p.max_len); }
 __device__ __forceinline__ int units_of_len(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
 
-// Range bounds floor(p * T / NP) = p * (T / NP) + floor(p * (T % NP) / NP); NP <= 4096 keeps the second product below 2^24.
+// The T units cut into NP = min(n_parts, T) ranges, none of them empty, with bounds floor(p * T / NP) = p * (T / NP) +
+// floor(p * (T % NP) / NP); NP <= 4096 keeps the second product below 2^24.
 struct Ranges {
   uint32_t np, tq, tr;
-  __device__ __forceinline__ Ranges(int t, int n) : np(n), tq((uint32_t)t / (uint32_t)n), tr((uint32_t)t % (uint32_t)n) {}
+  __device__ __forceinline__ Ranges(int t, int n_parts) {
+    np = (uint32_t)max(min(n_parts, t), 1);
+    tq = (uint32_t)t / np;
+    tr = (uint32_t)t % np;
+  }
   __device__ __forceinline__ int begin(int p) const { return (int)((uint32_t)p * tq + ((uint32_t)p * tr) / np); }
   // the last range that begins at or before unit u
   __device__ __forceinline__ int owner(int u) const {
-    const uint32_t t = tq * np + tr;
-    int p = (int)min((uint64_t)(np - 1), (uint64_t)u * np / t);
+    // a float estimate, put right by the bounds (u and np / T carry 24 bits: off by a few at most, whatever their sizes)
+    int p = min(max((int)((float)u * ((float)np / (float)(tq * np + tr))), 0), (int)np - 1);
+    while (p > 0 && begin(p) > u) --p;
     while (p + 1 < (int)np && begin(p + 1) <= u) ++p;
     return p;
   }
 };
 
-// Units of all sequences, and of those before sequence `b` if it is not negative (whole wave).
+// Units of all sequences, and of those before sequence `b` (whole wave).
 __device__ __forceinline__ int total_units(const Fp4Params& p, int b, int* before) {
   const int lane = threadIdx.x & 63;
   int sum = 0, pre = 0;
   for (int base = 0; base < p.batch; base += 64) {
-    const int i = base + lane, n = i < p.batch ? units_of_len(len_of(p, i)) : 0;
-    sum += n;
-    pre += i < b ? n : 0;
-  }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    sum += __shfl_xor(sum, m, 64);
-    pre += __shfl_xor(pre, m, 64);
+    const int n = base + lane < p.batch ? units_of_len(len_of(p, base + lane)) : 0, incl = wave_incl_scan(n);
+    if (b >= base && b < base + 64) pre = sum + __builtin_amdgcn_readlane(incl - n, b - base);
+    sum += __builtin_amdgcn_readlane(incl, 63);
   }
   *before = uni(pre);
   return uni(sum);
@@ -101,26 +103,27 @@ template <int SEL> __device__ __forceinline__ uint32_t widen2(uint32_t w, float 
   return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
 }
 
-// What a lane holds of one tile: K blocks (16 bytes each) with scale bytes, V dwords and scale words of its eight tokens.
-template <int D> struct TileRegs {
-  static constexpr int KB = D <= 128 ? 1 : 2;   // 32-element blocks of a K row per lane
-  static constexpr int VW = D <= 128 ? 1 : 2;   // dwords of a V row per lane (head dim 64: half a dword)
-  static constexpr int SW = D / 64;             // dwords that hold the V scales of two (64), one (128) or half a (256) token
-  u32x4 k[2][KB];
-  uint32_t ks[2][KB];
-  uint32_t v[8][VW];
-  uint32_t vs[2][4 * SW / 2];  // four tokens of D / 32 bytes
-};
+// (a constant-address-space load of a wave-uniform address is a scalar load: the block table does not pass through the
+// vector-memory counter, whose order the tile pipeline relies on)
+typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+__device__ __forceinline__ int scalar_load(const int32_t* p, int i) { return ((scalar_ptr)(uintptr_t)p)[i]; }
 
-template <typename QT, int D, int NRB, bool SOFTCAP>
+// Stream reads: a tile is read once per row group, and never again.
+template <typename T> __device__ __forceinline__ T stream_load(const uint8_t* p) { return __builtin_nontemporal_load((const T*)p); }
+
+// PT: a page holds whole tiles (its size is a multiple of kTile), else it holds whole blocks of sixteen tokens.
+template <typename QT, int D, int NRB, bool PT>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const Fp4Params p) {
   constexpr bool F16 = __is_same(QT, fp16_tag);
-  constexpr int KD = D <= 128 ? 1 : 2;          // 128-deep steps of Q.K^T
+  constexpr int KD = D <= 128 ? 1 : 2;          // 128-deep steps of Q.K^T = 32-element blocks of a K row per lane
   constexpr int NQ = F16 ? 3 : 2;               // e4m3 rows that add up to the query row
   constexpr int NQM = D == 64 ? (NQ + 1) / 2 : NQ;  // matrix operands of them (head dim 64: two rows side by side in the depth)
   constexpr int NP = F16 ? 2 : 1;               // bf16 parts of a probability
   constexpr int DPL = D / 16;                   // head elements per lane of the PV operand
-  using Regs = TileRegs<D>;
+  constexpr int VW = D <= 128 ? 1 : 2;          // dwords of them per token (head dim 64: half a dword)
+  constexpr int NB = kTile / 16;                // blocks of sixteen tokens in a tile
+  constexpr int NS = D / 32;                    // dwords that hold the scale bytes of four tokens
+  constexpr int ROW = D / 2;                    // bytes of a row of codes; its scale bytes are a sixteenth of that
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
   __shared__ float s_m[kWaves][16], s_l[kWaves][16];
 
@@ -131,48 +134,191 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   const int part = uni(pair / p.heads_kv), kvh = uni(pair - part * p.heads_kv);
   if (part >= p.n_parts) return;
 
-  int unused;
-  const int T = total_units(p, -1, &unused);
+  // Units of all sequences, this range of them, and its first sequence.  lens holds the lengths of sequences lens_base + lane:
+  // going on to the next sequence is a register read.
+  int T = 0, n0 = 0, incl0 = 0, lens = 0, lens_base = 0;
+  auto read_lens = [&](int base) __attribute__((always_inline)) -> int { return base + lane < p.batch ? len_of(p, base + lane) : 0; };
+  for (int base = 0; base < p.batch; base += 64) {
+    const int len = read_lens(base), n = units_of_len(len), incl = wave_incl_scan(n);
+    if (base == 0) {
+      lens = len;
+      n0 = n;
+      incl0 = incl;
+    }
+    T += __builtin_amdgcn_readlane(incl, 63);
+  }
+  T = uni(T);
   if (T == 0) return;
   const Ranges ranges(T, p.n_parts);
-  int u = uni(ranges.begin(part));
-  const int u_end = uni(ranges.begin(part + 1));
-  if (u >= u_end) return;
-
-  // first sequence of the range
-  int b = -1, pre = 0;
-  for (int base = 0, carry = 0; base < p.batch && b < 0; base += 64) {
-    const int i = base + lane, n = i < p.batch ? units_of_len(len_of(p, i)) : 0;
-    const int incl = wave_incl_scan(n);
-    const uint64_t hit = __ballot(carry + incl > u);
+  if (part >= (int)ranges.np) return;
+  const int u_begin = uni(ranges.begin(part)), u_end = uni(ranges.begin(part + 1));
+  int b_first = -1, pre_first = 0;
+  for (int base = 0, carry = 0; base < p.batch && b_first < 0; base += 64) {
+    int n = n0, incl = incl0;
+    if (base > 0) {
+      lens = read_lens(base);
+      lens_base = base;
+      n = units_of_len(lens);
+      incl = wave_incl_scan(n);
+    }
+    const uint64_t hit = __ballot(carry + incl > u_begin);
     if (hit) {
       const int at = uni(__ffsll((unsigned long long)hit) - 1);
-      b = base + at;
-      pre = carry + __builtin_amdgcn_readlane(incl - n, at);
+      b_first = base + at;
+      pre_first = carry + __builtin_amdgcn_readlane(incl - n, at);
     }
     carry += __builtin_amdgcn_readlane(incl, 63);
   }
-  b = uni(b);
-  pre = uni(pre);
 
   const int row0 = rg * 16 * NRB;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
-  const uint32_t page_rows = (uint32_t)p.page_size;
-  const bool causal = p.causal && p.q_len > 1;
-  const uint32_t v_shift = 8 * (D == 64 ? 0 : D == 128 ? c >> 2 : (c >> 1) & 3);
+  const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f;
+  const uint32_t q_sign = p.negate_q ? 0x80808080u : 0u;
+  // byte of the lane's block in a word of V scales (head dim 64: of the first of the word's two tokens), turned right by this
+  // many bits, sits in a float's exponent
+  const uint32_t v_turn = (8 * (D == 64 ? c >> 3 : D == 128 ? c >> 2 : (c >> 1) & 3) + 9) & 31;
+  // what the lane reads of a block of sixteen tokens: K row c, block g (head dim 64: g % 2); V rows 4g .. 4g + 3, elements c * DPL ..
+  const uint32_t k_lane = c * ROW + 16 * (D == 64 ? g & 1 : g), ks_lane = (D == 64 ? c & ~1 : c) * (ROW / 16);
+  const uint32_t k_shift = D == 64 ? 16 * (c & 1) + 8 * (g & 1) : 8 * g;  // of the lane's scale byte in the word it reads
+  const uint32_t v_lane = 4 * g * ROW + c * (DPL / 2), vs_lane = 4 * g * (ROW / 16);
+  const uint32_t page_bytes = (uint32_t)p.heads_kv * p.page_size * ROW;  // (below 2^32: the launcher checks)
+  const int64_t head_bytes = (int64_t)kvh * p.page_size * ROW;
 
-  for (int seg = 0; u < u_end; seg++) {
-    // ---- one sequence of the range --------------------------------------------------------------------------------
-    int len = uni(len_of(p, b));
-    while (len == 0) len = uni(len_of(p, ++b));  // (u < T: a sequence with tokens follows)
-    const int nu = units_of_len(len);
-    const int seg_u0 = u - pre, seg_u1 = min(nu, u_end - pre);  // units of the sequence
-    const bool whole = seg_u0 == 0 && seg_u1 == nu;
+  // One sequence of the range: units [u0, u1) of its nu; the wave's tiles are tok, tok + kUnit, .. below tok_end.
+  struct Segment {
+    int b, len, pre, nu, u0, u1, limit_min, tok, tok_end, last_page;
+  };
+  // The segment that begins at unit u, whose sequence is b0 or the first one behind it with tokens; pre: units before that.
+  auto segment_at = [&](int b0, int pre, int u) __attribute__((always_inline)) -> Segment {
+    Segment s;
+    s.b = b0;
+    while (true) {  // (u is below the number of units: there is such a sequence)
+      if (s.b < lens_base || s.b - lens_base >= 64) {  // (requests run ahead of the products)
+        lens_base = s.b;
+        lens = read_lens(s.b);
+      }
+      s.len = __builtin_amdgcn_readlane(lens, s.b - lens_base);
+      if (s.len > 0) break;
+      s.b++;
+    }
+    s.last_page = (s.len - 1) / p.page_size;
+    s.pre = pre;
+    s.nu = units_of_len(s.len);
+    s.u0 = u - pre;
+    s.u1 = min(s.nu, u_end - pre);
+    // tokens that the first and the last row of the group see; no row sees one past the latter
+    const int r_last = min(row0 + 16 * NRB, p.rows) - 1;
+    s.limit_min = causal ? s.len - p.q_len + row0 / p.group + 1 : s.len;
+    s.tok = s.u0 * kUnit + wave * kTile;
+    s.tok_end = min(s.u1 * kUnit, causal ? s.len - p.q_len + r_last / p.group + 1 : s.len);
+    return s;
+  };
+  Segment cur = segment_at(uni(b_first), uni(pre_first), u_begin);
 
-    // query rows: scaled by a power of two that puts the row's largest magnitude in [128, 256), then taken apart into e4m3 rows
-    u32x4 qf[NRB][KD][NQM][2];
-    float q_scale[NRB];
-    int limit[NRB], limit_min = INT_MAX, limit_max = 0;
+  // ---- requests: the wave's tiles of all segments as one stream, one tile ahead of the products, table entries one further ----
+  constexpr int NPG = PT ? 1 : NB;  // table entries of a tile
+  const int step_lp = kUnit / p.page_size, step_off = kUnit - step_lp * p.page_size;
+  Segment rq = cur;                // segment of the tile that is requested next,
+  int rq_tok, rq_lp, rq_off;       // its first token, and that one's logical page and offset
+  bool live = true;                // there is such a tile
+  int id[NPG], id_off[NPG];        // its table entries and the offsets of its blocks
+  auto rq_enter = [&]() __attribute__((always_inline)) {
+    rq_tok = rq.tok;
+    rq_lp = rq_tok / p.page_size;
+    rq_off = rq_tok - rq_lp * p.page_size;
+  };
+  auto rq_settle = [&]() __attribute__((always_inline)) {  // on to a segment that has a tile for this wave
+    while (rq_tok >= rq.tok_end) {
+      const int u_next = rq.pre + rq.nu;
+      if (u_next >= u_end) {
+        live = false;
+        return;
+      }
+      rq = segment_at(rq.b + 1, u_next, u_next);
+      rq_enter();
+    }
+    const int32_t* row = p.block_table + (int64_t)rq.b * p.bt_row_stride;
+    int lp = rq_lp, off = rq_off;
+#pragma unroll
+    for (int i = 0; i < NPG; i++) {
+      id[i] = scalar_load(row, min(lp, rq.last_page));  // (past the sequence's end: its last page again)
+      id_off[i] = off;
+      off += 16;
+      if (off == p.page_size) {
+        off = 0;
+        lp++;
+      }
+    }
+  };
+  int64_t at[NPG];  // byte offset of each block of the requested tile in the codes
+  auto rq_next = [&]() __attribute__((always_inline)) {
+    if (!live) return;  // (the last tile is requested again: the count of loads in flight stays the same)
+#pragma unroll
+    for (int i = 0; i < NPG; i++) {
+      const uint32_t page = (uint32_t)min(max(id[i], 0), p.n_pages - 1);
+      at[i] = (int64_t)((uint64_t)page * page_bytes) + head_bytes + id_off[i] * ROW;
+    }
+    rq_tok += kUnit;
+    rq_lp += step_lp;
+    rq_off += step_off;
+    if (rq_off >= p.page_size) {
+      rq_off -= p.page_size;
+      rq_lp++;
+    }
+    rq_settle();
+  };
+  u32x4 kr[NB][KD];
+  uint32_t ksr[NB][KD], vr[NB][4][VW], vsr[NB][NS];
+  auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      const int64_t o = PT ? at[0] + i * 16 * ROW : at[PT ? 0 : i];
+      const uint8_t *kp = p.k + o, *ksp = p.k_scale + (o >> 4);
+#pragma unroll
+      for (int kd = 0; kd < KD; kd++) {
+        kr[i][kd] = stream_load<u32x4>(kp + k_lane + 64 * kd);
+        ksr[i][kd] = stream_load<uint32_t>(ksp + ks_lane + 4 * kd);  // (shifted down at its use: nothing may touch it here)
+      }
+    }
+  };
+  auto load_v = [&](int i) __attribute__((always_inline)) {
+    const int64_t o = PT ? at[0] + i * 16 * ROW : at[PT ? 0 : i];
+    const uint8_t *vp = p.v + o, *vsp = p.v_scale + (o >> 4);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (D == 64) vr[i][j][0] = stream_load<uint16_t>(vp + v_lane + j * ROW);
+      else if constexpr (D == 128) vr[i][j][0] = stream_load<uint32_t>(vp + v_lane + j * ROW);
+      else {
+        const u32x2 w = stream_load<u32x2>(vp + v_lane + j * ROW);
+        vr[i][j][0] = w[0];
+        vr[i][j][1] = w[1];
+      }
+    }
+    if constexpr (NS == 2) {
+      const u32x2 w = stream_load<u32x2>(vsp + vs_lane);
+      vsr[i][0] = w[0];
+      vsr[i][1] = w[1];
+    } else {
+#pragma unroll
+      for (int h = 0; h < NS / 4; h++) {
+        const u32x4 w = stream_load<u32x4>(vsp + vs_lane + 16 * h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) vsr[i][4 * h + e] = w[e];
+      }
+    }
+  };
+  rq_enter();
+  rq_settle();
+  if (live) {
+    rq_next();
+    load_k();
+#pragma unroll
+    for (int i = 0; i < NB; i++) load_v(i);
+  }
+
+  // query rows of a sequence, as they are; the next sequence's are requested before this one's results are joined
+  u32x4 q_raw[NRB][D / 64][2];
+  auto load_q = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int rb = 0; rb < NRB; rb++) {
       const int r = row0 + 16 * rb + c;
@@ -180,15 +326,37 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       const int s = valid ? r / p.group : 0, gi = valid ? r - s * p.group : 0;
       const uint16_t* qp = p.q + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D;
       // depth positions of the lane's sixteen-byte halves h: [64h + 16g, 64h + 16g + 16) of each 128-deep step
+#pragma unroll
+      for (int h = 0; h < D / 64; h++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          q_raw[rb][h][e] = u32x4{0, 0, 0, 0};
+          if (valid) q_raw[rb][h][e] = *(const u32x4*)(qp + 64 * h + 16 * g + 8 * e);
+        }
+    }
+  };
+  load_q(cur.b);
+
+  for (int seg = 0;; seg++) {
+    // ---- one sequence of the range --------------------------------------------------------------------------------
+    const int b = cur.b, len = cur.len, limit_min = cur.limit_min, tok_end = cur.tok_end;
+    const bool whole = cur.u0 == 0 && cur.u1 == cur.nu;
+    int tok = cur.tok;
+
+    // query rows: scaled by a power of two that puts the row's largest magnitude in [128, 256), then taken apart into e4m3 rows
+    u32x4 qf[NRB][KD][NQM][2];
+    float q_scale[NRB];
+    int limit[NRB];
+#pragma unroll
+    for (int rb = 0; rb < NRB; rb++) {
+      const int r = row0 + 16 * rb + c;
       constexpr int NH = D / 64;
       float f[16 * NH];
 #pragma unroll
       for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          u32x4 raw = {0, 0, 0, 0};
-          if (valid) raw = *(const u32x4*)(qp + 64 * h + 16 * g + 8 * e);
-          const uint32_t w[4] = {raw[0], raw[1], raw[2], raw[3]};
+          const uint32_t w[4] = {q_raw[rb][h][e][0], q_raw[rb][h][e][1], q_raw[rb][h][e][2], q_raw[rb][h][e][3]};
           Unpack<QT, 8>::run(w, f + 16 * h + 8 * e);
         }
       float am = 0.f;
@@ -199,6 +367,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       float inv = __uint_as_float((261u - be) << 23);  // 2^(7 - e)
       q_scale[rb] = __uint_as_float((be - 7u) << 23);
       if (be == 255u) inv = q_scale[rb] = __builtin_nanf("");  // an infinity in the row: its scores are not numbers
+      if (!softcap) q_scale[rb] *= p.score_scale;
       u32x4 parts[NH][NQ];
 #pragma unroll
       for (int h = 0; h < NH; h++)
@@ -215,7 +384,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
             a[1] -= lo[1];
             a[2] -= hi[0];
             a[3] -= hi[1];
-            parts[h][n][w] = word;
+            parts[h][n][w] = word ^ q_sign;
           }
         }
       if constexpr (D == 64) {
@@ -233,222 +402,193 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
 #pragma unroll
             for (int h = 0; h < 2; h++) qf[rb][kd][n][h] = parts[2 * kd + h][n];
       }
-      limit[rb] = valid ? (causal ? len - p.q_len + s + 1 : len) : 0;
-    }
-    {
-      // tokens that the first and the last row of the group see (uniform)
-      const int r_last = min(row0 + 16 * NRB, p.rows) - 1;
-      limit_min = causal ? len - p.q_len + row0 / p.group + 1 : len;
-      limit_max = causal ? len - p.q_len + r_last / p.group + 1 : len;
-      limit_min = uni(limit_min);
-      limit_max = uni(limit_max);
+      limit[rb] = r < p.rows ? (causal ? len - p.q_len + r / p.group + 1 : len) : 0;
     }
 
-    f32x4 o[NRB][DPL];
-    float m_run[NRB], l_run[NRB];
+    f32x4 o[NRB][DPL], lsum[NRB];  // (lsum: four equal copies of the row's sum)
+    float m_run[NRB];
 #pragma unroll
     for (int rb = 0; rb < NRB; rb++) {
       m_run[rb] = kNegFloor;
-      l_run[rb] = 0.f;
+      lsum[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < DPL; n++) o[rb][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    constexpr uint32_t kOnes = 0x3f803f80u;  // two bf16 ones
 
-    // ---- the wave's tiles -------------------------------------------------------------------------------------------
-    const int tok_end = min(seg_u1 * kUnit, limit_max);  // tokens past it no row of the group sees
-    int tok = seg_u0 * kUnit + wave * kTile;
-    const int32_t* bt_row = p.block_table + (int64_t)b * p.bt_row_stride;
-    const int last_page = (len - 1) / p.page_size;
-    // rows of the pool (of this kv head) that hold the two sixteen-token halves of a tile
-    auto pool_row = [&](int t) __attribute__((always_inline)) -> int64_t {
-      const int lp = min(t / p.page_size, last_page), off = t % p.page_size;
-      const int page = min(max(bt_row[lp], 0), p.n_pages - 1);
-      return ((int64_t)page * p.heads_kv + kvh) * page_rows + off;
+    // scale of token 4g + j of block i for the lane's head elements: its byte turned to a float's exponent (255 reads as NaN)
+    auto v_scale = [&](int i, int j) __attribute__((always_inline)) -> uint32_t {
+      const uint32_t w = D == 64 ? vsr[i][j >> 1] : D == 128 ? vsr[i][j] : c & 8 ? vsr[i][NS > 4 ? 2 * j + 1 : 0] : vsr[i][NS > 4 ? 2 * j : 0];
+      return __builtin_amdgcn_alignbit(w, w, D == 64 && (j & 1) ? (v_turn + 16) & 31 : v_turn) & 0x7f800000u;
     };
-    auto load = [&](int t, Regs& r) __attribute__((always_inline)) {
+    // A operands of the PV product for two head elements at a time: word_of(j, w) is the pair w of token j (0..7) as two bf16
+    auto value_operands = [&](auto word_of, auto use) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int64_t row = pool_row(t + 16 * i);
-        const uint8_t* kp = p.k + row * (D / 2);
-        const uint8_t* ksp = p.k_scale + row * (D / 32);
-        const uint8_t* vp = p.v + row * (D / 2);
-        const uint8_t* vsp = p.v_scale + row * (D / 32);
+      for (int w = 0; w < DPL / 2; w++) {
+        uint32_t e8[8];
 #pragma unroll
-        for (int kb = 0; kb < Regs::KB; kb++) {
-          const int block = D == 64 ? (g & 1) : 4 * kb + g;
-          r.k[i][kb] = *(const u32x4*)(kp + c * (D / 2) + 16 * block);
-          r.ks[i][kb] = ksp[c * (D / 32) + block];
+        for (int j = 0; j < 8; j++) e8[j] = word_of(j, w);
+        u32x4 lo, hi;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          lo[k] = __builtin_amdgcn_perm(e8[2 * k + 1], e8[2 * k], 0x05040100u);
+          hi[k] = __builtin_amdgcn_perm(e8[2 * k + 1], e8[2 * k], 0x07060302u);
         }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint8_t* vr = vp + (4 * g + j) * (D / 2) + c * (DPL / 2);
-          if constexpr (D == 64) r.v[4 * i + j][0] = *(const uint16_t*)vr;
-          else if constexpr (D == 128) r.v[4 * i + j][0] = *(const uint32_t*)vr;
-          else {
-            const u32x2 w = *(const u32x2*)vr;
-            r.v[4 * i + j][0] = w[0];
-            r.v[4 * i + j][1] = w[1];
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4 * Regs::SW / 2; j++) r.vs[i][j] = ((const uint32_t*)(vsp + 4 * g * (D / 32)))[j];
+        use(2 * w, lo);
+        use(2 * w + 1, hi);
       }
     };
-    // scale of token j (0..7) for the lane's head elements: its byte in place of a float's exponent (255 reads as NaN)
-    auto v_byte = [&](const Regs& r, int j) __attribute__((always_inline)) -> uint32_t {
-      const int i = j >> 2, jj = j & 3;
-      uint32_t w;
-      if constexpr (D == 64) w = r.vs[i][jj >> 1] >> (16 * (jj & 1) + 8 * (c >> 3));
-      else if constexpr (D == 128) w = r.vs[i][jj] >> v_shift;
-      else w = (c & 8 ? r.vs[i][2 * jj + 1] : r.vs[i][2 * jj]) >> v_shift;
-      return w & 0xffu;
-    };
 
-    auto step = [&](const Regs& r, int t) __attribute__((always_inline)) {
-      const bool masked = t + kTile > limit_min;
-      uint32_t pw[NRB][NP][4];
-      uint32_t seen_bits[NRB];
+    // One tile.  The registers of K are free once its products are issued, those of V once it is widened: the next tile is
+    // requested there, so a tile's reads have the rest of the step and the head of the next one to arrive.
+    auto step = [&](auto masked_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      f32x4 s[NRB][NB];
 #pragma unroll
-      for (int rb = 0; rb < NRB; rb++) {
-        f32x4 s[2];
+      for (int rb = 0; rb < NRB; rb++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < NB; i++) {
+          s[rb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kd = 0; kd < KD; kd++) {
-            const u32x4 kk = r.k[i][kd];
+            const u32x4 kk = kr[i][kd];
             const i32x8 a = {(int)kk[0], (int)kk[1], (int)kk[2], (int)kk[3], 0, 0, 0, 0};
 #pragma unroll
             for (int n = 0; n < NQM; n++) {
               const u32x4 b0 = qf[rb][kd][n][0], b1 = qf[rb][kd][n][1];
               const i32x8 bq = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
-              acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bq, acc, 4, 0, 0, (int)r.ks[i][kd], 0, 127);
+              s[rb][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bq, s[rb][i], 4, 0, 0, (int)(ksr[i][kd] >> k_shift), 0, 127);
             }
           }
-          s[i] = acc;
         }
-        float z[8];
-        seen_bits[rb] = 0xffu;
+      __builtin_amdgcn_sched_barrier(0);
+      rq_next();
+      load_k();
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t pw[NRB][NB / 2][NP][4], seen_bits[NRB][NB / 2];
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          z[e] = to_logit2<SOFTCAP>(s[e >> 2][e & 3] * q_scale[rb], p.score_scale, p.cap_log2e, p.inv_cap_scale);
-        if (masked) {
-          seen_bits[rb] = 0;
+      for (int rb = 0; rb < NRB; rb++) {
+        float f = q_scale[rb];
+        if (softcap) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const bool seen = t + 16 * (e >> 2) + 4 * g + (e & 3) < limit[rb];
-            z[e] = seen ? z[e] : -INFINITY;
-            seen_bits[rb] |= seen ? 1u << e : 0u;
+          for (int e = 0; e < 4 * NB; e++) s[rb][e >> 2][e & 3] = to_logit2<true>(s[rb][e >> 2][e & 3] * f, 0.f, p.cap_log2e, p.inv_cap_scale);
+          f = 1.f;
+        }
+        float top;
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int h = 0; h < NB / 2; h++) seen_bits[rb][h] = 0;
+#pragma unroll
+          for (int e = 0; e < 4 * NB; e++) {
+            const bool seen = tok + 16 * (e >> 2) + 4 * g + (e & 3) < limit[rb];
+            s[rb][e >> 2][e & 3] = seen ? s[rb][e >> 2][e & 3] * f : -INFINITY;
+            seen_bits[rb][e >> 3] |= seen ? 1u << (e & 7) : 0u;
           }
+          f = 1.f;
         }
-        float top = max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), max2(z[6], z[7]));
-        top = group_max(top);
+        // (med3 with +inf is a maximum that the compiler schedules behind the matrix results, without quieting its operands first)
+        top = __builtin_amdgcn_fmed3f(s[rb][0][0], s[rb][0][1], INFINITY);
+#pragma unroll
+        for (int e = 2; e < 4 * NB; e++) top = __builtin_amdgcn_fmed3f(top, s[rb][e >> 2][e & 3], INFINITY);
+        top = group_max(top) * f;  // (f >= 0: the sign of the softmax scale is in the query)
         if (__ballot(top > m_run[rb] + kRescaleGap4)) {  // (the first tile with a visible token always comes here)
           const float m_new = top > m_run[rb] + kRescaleGap4 ? top : m_run[rb];
-          const float f = fast_exp2(m_run[rb] - m_new);
+          const float shrink = fast_exp2(m_run[rb] - m_new);
           m_run[rb] = m_new;
-          l_run[rb] *= f;
+          lsum[rb] *= shrink;
 #pragma unroll
-          for (int n = 0; n < DPL; n++) o[rb][n] *= f;
+          for (int n = 0; n < DPL; n++) o[rb][n] *= shrink;
         }
-        float pr[8], sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          pr[e] = fast_exp2(z[e] - m_run[rb]);
-          sum += pr[e];
-        }
-        l_run[rb] += sum;
+        for (int h = 0; h < NB / 2; h++) {
+          float pr[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          pw[rb][0][e] = pack_bf16(pr[2 * e], pr[2 * e + 1]);
-          if constexpr (NP == 2)
-            pw[rb][1][e] = pack_bf16(pr[2 * e] - __uint_as_float(pw[rb][0][e] << 16), pr[2 * e + 1] - __uint_as_float(pw[rb][0][e] & 0xffff0000u));
-        }
-      }
-      float vsc[8];
-      uint32_t bad = 0;  // tokens (bits) whose block is NaN
+          for (int e = 0; e < 8; e++) pr[e] = fast_exp2(__builtin_fmaf(s[rb][2 * h + (e >> 2)][e & 3], f, -m_run[rb]));
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const uint32_t byte = v_byte(r, j);
-        vsc[j] = __uint_as_float(byte << 23);
-        if (masked) {
-          // a NaN block stays out of the product, where a weight of zero would not keep it from the rows that do not see it
-          bad |= byte == 255u ? 1u << j : 0u;
-          vsc[j] = byte == 255u ? 0.f : vsc[j];
-        }
-      }
-      auto value_step = [&](auto word_of, auto use) __attribute__((always_inline)) {
-#pragma unroll
-        for (int w = 0; w < (DPL + 1) / 2; w++) {  // two head elements of the lane at a time
-          uint32_t e8[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) e8[j] = word_of(j, w);
-          u32x4 lo, hi;
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            lo[k] = __builtin_amdgcn_perm(e8[2 * k + 1], e8[2 * k], 0x05040100u);
-            hi[k] = __builtin_amdgcn_perm(e8[2 * k + 1], e8[2 * k], 0x07060302u);
+          for (int e = 0; e < 4; e++) {
+            pw[rb][h][0][e] = pack_bf16(pr[2 * e], pr[2 * e + 1]);
+            if constexpr (NP == 2)
+              pw[rb][h][1][e] = pack_bf16(pr[2 * e] - __uint_as_float(pw[rb][h][0][e] << 16), pr[2 * e + 1] - __uint_as_float(pw[rb][h][0][e] & 0xffff0000u));
           }
-          use(2 * w, lo);
-          use(2 * w + 1, hi);
+          // the row's sum of the probabilities as rounded, on the matrix unit: every row of ones . P^T
+#pragma unroll
+          for (int q = 0; q < NP; q++)
+            lsum[rb] = mma_bf16(u32x4{kOnes, kOnes, kOnes, kOnes}, u32x4{pw[rb][h][q][0], pw[rb][h][q][1], pw[rb][h][q][2], pw[rb][h][q][3]}, lsum[rb]);
         }
-      };
-      value_step(
-          [&](int j, int w) __attribute__((always_inline)) -> uint32_t {
-            const uint32_t word = r.v[j][w >> 2];
-            switch (w & 3) {
-              case 0: return widen2<0>(word, vsc[j]);
-              case 1: return widen2<1>(word, vsc[j]);
-              case 2: return widen2<2>(word, vsc[j]);
-              default: return widen2<3>(word, vsc[j]);
+      }
+#pragma unroll
+      for (int h = 0; h < NB / 2; h++) {
+        float vsc[8];
+        uint32_t bad = 0;  // tokens (bits) whose block is NaN
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const uint32_t expo = v_scale(2 * h + (j >> 2), j & 3);
+          vsc[j] = __uint_as_float(expo);
+          if constexpr (MASKED) {
+            // a NaN block stays out of the product, where a weight of zero would not keep it from the rows that do not see it
+            bad |= expo == 0x7f800000u ? 1u << j : 0u;
+            vsc[j] = expo == 0x7f800000u ? 0.f : vsc[j];
+          }
+        }
+        value_operands(
+            [&](int j, int w) __attribute__((always_inline)) -> uint32_t {
+              const uint32_t word = vr[2 * h + (j >> 2)][j & 3][w >> 2];
+              switch (w & 3) {
+                case 0: return widen2<0>(word, vsc[j]);
+                case 1: return widen2<1>(word, vsc[j]);
+                case 2: return widen2<2>(word, vsc[j]);
+                default: return widen2<3>(word, vsc[j]);
+              }
+            },
+            [&](int n, u32x4 a) __attribute__((always_inline)) {
+#pragma unroll
+              for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+                for (int q = 0; q < NP; q++)
+                  o[rb][n] = mma_bf16(a, u32x4{pw[rb][h][q][0], pw[rb][h][q][1], pw[rb][h][q][2], pw[rb][h][q][3]}, o[rb][n]);
+            });
+        if constexpr (MASKED) {
+          if (__ballot(bad != 0u)) {
+            // rows that see a token with a NaN block get NaN there: count such tokens with the same product, 1 for every
+            // NaN block against 1 for every visible token
+#pragma unroll
+            for (int rb = 0; rb < NRB; rb++) {
+              u32x4 vis;
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                vis[k] = ((seen_bits[rb][h] >> (2 * k)) & 1u ? 0x3f80u : 0u) | ((seen_bits[rb][h] >> (2 * k + 1)) & 1u ? 0x3f800000u : 0u);
+              value_operands([&](int j, int) __attribute__((always_inline)) -> uint32_t { return (bad >> j) & 1u ? kOnes : 0u; },
+                             [&](int n, u32x4 a) __attribute__((always_inline)) {
+                               const f32x4 count = mma_bf16(a, vis, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                               for (int i = 0; i < 4; i++) o[rb][n][i] = count[i] > 0.f ? __builtin_nanf("") : o[rb][n][i];
+                             });
             }
-          },
-          [&](int n, u32x4 a) __attribute__((always_inline)) {
-#pragma unroll
-            for (int rb = 0; rb < NRB; rb++)
-#pragma unroll
-              for (int q = 0; q < NP; q++) o[rb][n] = mma_bf16(a, u32x4{pw[rb][q][0], pw[rb][q][1], pw[rb][q][2], pw[rb][q][3]}, o[rb][n]);
-          });
-      if (masked && __ballot(bad != 0u)) {
-        // rows that see a token with a NaN block get NaN there: count such tokens with the same product, 1 for every
-        // NaN block against 1 for every visible token
-#pragma unroll
-        for (int rb = 0; rb < NRB; rb++) {
-          u32x4 vis;
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            vis[k] = ((seen_bits[rb] >> (2 * k)) & 1u ? 0x3f80u : 0u) | ((seen_bits[rb] >> (2 * k + 1)) & 1u ? 0x3f800000u : 0u);
-          value_step([&](int j, int) __attribute__((always_inline)) -> uint32_t { return (bad >> j) & 1u ? 0x3f803f80u : 0u; },
-                     [&](int n, u32x4 a) __attribute__((always_inline)) {
-                       const f32x4 count = mma_bf16(a, vis, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                       for (int i = 0; i < 4; i++) o[rb][n][i] = count[i] > 0.f ? __builtin_nanf("") : o[rb][n][i];
-                     });
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(2 * h);
+        load_v(2 * h + 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
+    for (; tok + kTile <= limit_min && tok < tok_end; tok += kUnit) step(std::false_type{});
+    for (; tok < tok_end; tok += kUnit) step(std::true_type{});
 
-    if (tok < tok_end) {
-      Regs cur;
-      load(tok, cur);
-      while (true) {
-        const int next = tok + kUnit;
-        Regs ahead;
-        if (next < tok_end) load(next, ahead);
-        step(cur, tok);
-        if (next >= tok_end) break;
-        cur = ahead;
-        tok = next;
-      }
+    const int u_next = cur.pre + cur.nu;
+    const bool last = u_next >= u_end;
+    Segment next = cur;
+    if (!last) {
+      next = segment_at(b + 1, u_next, u_next);
+      load_q(next.b);
     }
 
     // ---- the four waves' results of each block of rows meet in LDS ---------------------------------------------------
 #pragma unroll
     for (int rb = 0; rb < NRB; rb++) {
-      const float l_all = group_sum(l_run[rb]);
       if (g == 0) {
         s_m[wave][c] = m_run[rb];
-        s_l[wave][c] = l_all;
+        s_l[wave][c] = lsum[rb][0];
       }
       // lane (c, g) holds head elements (D / 4) * g + DPL * i + n of row c
 #pragma unroll
@@ -494,74 +634,73 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       }
       __syncthreads();
     }
-    u = pre + seg_u1;
-    pre += nu;
-    if (u == pre) ++b;
-    else pre -= nu;
+    if (last) return;
+    cur = next;
   }
 }
 
-// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  One wave per row.
-// Sequences without tokens get zeros here.
+// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  One wave per row, a
+// lane has four head elements, so the 64 / (D / 4) lane groups of a wave take different ranges; eight loads of each group are in
+// flight before the first weight is known.  Sequences without tokens get zeros here.
 template <typename QT, int D>
 __global__ __launch_bounds__(256) void paged_decode_fp4_merge_kernel(const Fp4Params p) {
-  const int lane = threadIdx.x & 63, b = blockIdx.y;
+  constexpr int LPR = D / 4, GROUPS = 64 / LPR, PRE = 8;  // lanes per row, ranges side by side, loads in flight
+  const int lane = threadIdx.x & 63, b = blockIdx.y, grp = lane / LPR, d0 = 4 * (lane % LPR);
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
   const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
-  const int nu = uni(units_of_len(len_of(p, b)));
   int pre;
   const int T = total_units(p, b, &pre);
-  int p_first = 0, p_last = -1;
+  const int nu = uni(units_of_len(len_of(p, b)));
+  int first = 0, last = -1;
   bool second = false;
   const Ranges ranges(T, p.n_parts);
   if (nu > 0) {
-    p_first = uni(ranges.owner(pre));
-    p_last = uni(ranges.owner(pre + nu - 1));
-    if (p_first == p_last) return;  // written by the range that holds it
-    second = ranges.begin(p_first) != pre;
+    first = uni(ranges.owner(pre));
+    last = uni(ranges.owner(pre + nu - 1));
+    if (first == last) return;  // written by the range that holds it
+    second = ranges.begin(first) != pre;
   }
   if (row >= rows_all) return;
-  const int kvh = (int)(row / p.rows), r = (int)(row - (int64_t)kvh * p.rows), s = r / p.group, gi = r - s * p.group;
-  constexpr int E = D / 64;
-  float acc[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) acc[e] = 0.f;
-  auto slot_of = [&](int part) { return (int64_t)(2 * part + (part == p_first && second ? 1 : 0)) * rows_all + row; };
+  const int n = last - first + 1;
+  auto slot_of = [&](int i) __attribute__((always_inline)) -> int64_t {
+    const int part = first + min(i, n - 1);
+    return (int64_t)(2 * part + (part == first && second ? 1 : 0)) * rows_all + row;
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float M = -INFINITY, W = 0.f;
-  for (int base = p_first; base <= p_last; base += 64) {
-    const int part = base + lane;
-    // (a range can be empty when there are fewer units than ranges: it wrote nothing)
-    const bool there = part <= p_last && ranges.begin(part) < ranges.begin(part + 1);
-    const float lse = there ? p.part_lse[slot_of(part)] : -INFINITY;
-    float top = fmaxf(lse, __shfl_xor(lse, 1, 64));
+  for (int base = 0; base < n; base += PRE * GROUPS) {
+    f32x4 x[PRE];
 #pragma unroll
-    for (int m = 2; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    const float M_new = fmaxf(M, top);
-    if (__ballot(lse != lse)) W = __builtin_nanf("");
-    if (M_new == -INFINITY) continue;
-    const float f = fast_exp2(M - M_new), wl = there ? fast_exp2(lse - M_new) : 0.f;
-    W *= f;
+    for (int i = 0; i < PRE; i++) x[i] = *(const f32x4*)(p.part_o + slot_of(base + i * GROUPS + grp) * D + d0);
+    const bool there = lane < PRE * GROUPS && base + lane < n;
+    const float lse = there ? p.part_lse[slot_of(base + lane)] : -INFINITY;
+    float top = lse;
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[e] *= f;
-    M = M_new;
-    const int n = min(64, p_last - base + 1);
-    for (int i = 0; i < n; i++) {
-      const float w = __shfl(wl, i, 64);
-      if (w == 0.f) continue;  // (a slot that nothing was written to may hold anything)
-      const float* src = p.part_o + slot_of(base + i) * D + E * lane;
+    for (int m = 1; m < PRE * GROUPS; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    top = fmaxf(M, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, top), 0)));
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float shrink = fast_exp2(M - ref), wl = fast_exp2(lse - ref);  // (NaN stays NaN)
+    M = top;
+    W *= shrink;
+    acc *= shrink;
+#pragma unroll
+    for (int i = 0; i < PRE; i++) {
+      const float w = __shfl(wl, i * GROUPS + grp, 64);
       W += w;
-#pragma unroll
-      for (int e = 0; e < E; e++) acc[e] += w * src[e];
+      if (w != 0.f) acc += w * x[i];  // (a row that saw nothing holds zeros, and a place past the last is not added)
     }
   }
-  const float inv = W == 0.f ? 0.f : 1.0f / W;
-  uint16_t* dst = p.out + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D + E * lane;
-  if constexpr (E == 1) {
-    dst[0] = (uint16_t)(pack16<QT>(acc[0] * inv, 0.f) & 0xffffu);
-  } else {
 #pragma unroll
-    for (int e = 0; e < E; e += 2) *(uint32_t*)(dst + e) = pack16<QT>(acc[e] * inv, acc[e + 1] * inv);
+  for (int m = LPR; m < 64; m <<= 1) {
+    W += __shfl_xor(W, m, 64);
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], m, 64);
   }
+  if (grp > 0) return;
+  const float inv = W == 0.f ? 0.f : 1.0f / W;
+  const int kvh = (int)(row / p.rows), r = (int)(row - (int64_t)kvh * p.rows), s = r / p.group, gi = r - s * p.group;
+  *(u32x2*)(p.out + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D + d0) =
+      u32x2{pack16<QT>(acc[0] * inv, acc[1] * inv), pack16<QT>(acc[2] * inv, acc[3] * inv)};
 }
 
 constexpr int kMaxParts4 = 4096;
@@ -572,11 +711,11 @@ int row_blocks(int rows, int dim) { return rows <= 16 || dim == 256 ? 1 : 2; }
 int row_groups_of(int rows, int dim) { return (rows + 16 * row_blocks(rows, dim) - 1) / (16 * row_blocks(rows, dim)); }
 
 template <typename QT, int D, int NRB>
-const char* launch_fp4(const Fp4Params& p, bool softcap, hipStream_t s) {
+const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
   const int64_t pairs = (int64_t)p.n_parts * p.heads_kv;
   const int64_t grid = 8 * (int64_t)p.row_groups * ((pairs + 7) / 8);
   if (grid > INT_MAX) return "too many workgroups";
-  if (softcap)
+  if (p.page_size % kTile == 0)
     hipLaunchKernelGGL((paged_decode_fp4_kernel<QT, D, NRB, true>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, p);
   else
     hipLaunchKernelGGL((paged_decode_fp4_kernel<QT, D, NRB, false>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, p);
@@ -589,16 +728,16 @@ const char* launch_fp4(const Fp4Params& p, bool softcap, hipStream_t s) {
 }
 
 template <typename QT>
-const char* launch_fp4_dim(const Fp4Params& p, int dim, bool softcap, hipStream_t s) {
+const char* launch_fp4_dim(const Fp4Params& p, int dim, hipStream_t s) {
   const bool one = row_blocks(p.rows, dim) == 1;
-  if (dim == 64) return one ? launch_fp4<QT, 64, 1>(p, softcap, s) : launch_fp4<QT, 64, 2>(p, softcap, s);
-  if (dim == 128) return one ? launch_fp4<QT, 128, 1>(p, softcap, s) : launch_fp4<QT, 128, 2>(p, softcap, s);
-  return launch_fp4<QT, 256, 1>(p, softcap, s);
+  if (dim == 64) return one ? launch_fp4<QT, 64, 1>(p, s) : launch_fp4<QT, 64, 2>(p, s);
+  if (dim == 128) return one ? launch_fp4<QT, 128, 1>(p, s) : launch_fp4<QT, 128, 2>(p, s);
+  return launch_fp4<QT, 256, 1>(p, s);
 }
 
 }  // namespace
 
-// Ranges of the token stream: two workgroups (eight waves) per compute unit over all (kv head, row group) pairs.
+// Ranges of the token stream: two workgroups (eight waves) per compute unit, over all (kv head, row group) pairs.
 int fp4_num_parts(int heads_kv, int rows, int dim, int compute_units) {
   const int64_t parts = 2 * (int64_t)compute_units / ((int64_t)heads_kv * row_groups_of(rows, dim));
   return parts < 1 ? 1 : parts > kMaxParts4 ? kMaxParts4 : (int)parts;
@@ -642,11 +781,13 @@ const char* launch_decode_fp4(const void* q, const void* k, const void* v, const
   const size_t slots = (size_t)2 * n_parts * heads_kv * p.rows;
   p.part_o = (float*)workspace;
   p.part_lse = (float*)((char*)workspace + align256(slots * dim * sizeof(float)));
-  const bool cap_on = softcap > 0.f;
+  // the kernel takes maxima before it scales: the sign of the scale goes into the query
+  p.negate_q = sm_scale < 0.f;
+  sm_scale = fabsf(sm_scale);
   p.score_scale = sm_scale * kLog2e;
   p.cap_log2e = softcap * kLog2e;
-  p.inv_cap_scale = cap_on ? sm_scale / softcap : 0.f;
-  return q_dtype == MI355_DT_BF16 ? launch_fp4_dim<bf16_tag>(p, dim, cap_on, s) : launch_fp4_dim<fp16_tag>(p, dim, cap_on, s);
+  p.inv_cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f;
+  return q_dtype == MI355_DT_BF16 ? launch_fp4_dim<bf16_tag>(p, dim, s) : launch_fp4_dim<fp16_tag>(p, dim, s);
 }
 
 }  // namespace mi355

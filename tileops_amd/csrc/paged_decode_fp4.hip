@@ -45,7 +45,7 @@ struct Fp4Params {
   float *part_o, *part_lse;
   int batch, q_len, heads, heads_kv, page_size, group, rows, row_groups, n_parts, max_len, causal, negate_q;
   int n_pages;
-  float score_scale, cap_log2e, inv_cap_scale;
+  float score_scale, cap_log2e;  // scale of a score to its logit2, with a cap to 2 log2(e) times the tanh's argument
 };
 
 __device__ __forceinline__ int len_of(const Fp4Params& p, int b) { return min(max(p.seqlens[b], 0), p.max_len); }
@@ -221,11 +221,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   Segment rq = cur;                // segment of the tile that is requested next,
   int rq_tok, rq_lp, rq_off;       // its first token, and that one's logical page and offset
   bool live = true;                // there is such a tile
+  const int32_t* rq_row = p.block_table;  // its sequence's table row
   int id[NPG], id_off[NPG];        // its table entries and the offsets of its blocks
   auto rq_enter = [&]() __attribute__((always_inline)) {
     rq_tok = rq.tok;
     rq_lp = rq_tok / p.page_size;
     rq_off = rq_tok - rq_lp * p.page_size;
+    rq_row = p.block_table + (int64_t)rq.b * p.bt_row_stride;
   };
   auto rq_settle = [&]() __attribute__((always_inline)) {  // on to a segment that has a tile for this wave
     while (rq_tok >= rq.tok_end) {
@@ -237,11 +239,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       rq = segment_at(rq.b + 1, u_next, u_next);
       rq_enter();
     }
-    const int32_t* row = p.block_table + (int64_t)rq.b * p.bt_row_stride;
     int lp = rq_lp, off = rq_off;
 #pragma unroll
     for (int i = 0; i < NPG; i++) {
-      id[i] = scalar_load(row, min(lp, rq.last_page));  // (past the sequence's end: its last page again)
+      id[i] = scalar_load(rq_row, min(lp, rq.last_page));  // (past the sequence's end: its last page again)
       id_off[i] = off;
       off += 16;
       if (off == p.page_size) {
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       float inv = __uint_as_float((261u - be) << 23);  // 2^(7 - e)
       q_scale[rb] = __uint_as_float((be - 7u) << 23);
       if (be == 255u) inv = q_scale[rb] = __builtin_nanf("");  // an infinity in the row: its scores are not numbers
-      if (!softcap) q_scale[rb] *= p.score_scale;
+      q_scale[rb] *= p.score_scale;
       u32x4 parts[NH][NQ];
 #pragma unroll
       for (int h = 0; h < NH; h++)
@@ -466,44 +467,58 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       load_k();
       __builtin_amdgcn_sched_barrier(0);
       uint32_t pw[NRB][NB / 2][NP][4], seen_bits[NRB][NB / 2];
+      float slope[NRB], offset[NRB], top[NRB];  // logit = slope * s + offset, slope >= 0 (the sign of the softmax scale is in the query)
+      bool grown = false;
 #pragma unroll
       for (int rb = 0; rb < NRB; rb++) {
-        float f = q_scale[rb];
+        slope[rb] = q_scale[rb];
+        offset[rb] = 0.f;
         if (softcap) {
+          // cap * tanh(x) = cap - 2 cap / (exp(2x) + 1): s becomes -1 / (exp(2x) + 1)
 #pragma unroll
-          for (int e = 0; e < 4 * NB; e++) s[rb][e >> 2][e & 3] = to_logit2<true>(s[rb][e >> 2][e & 3] * f, 0.f, p.cap_log2e, p.inv_cap_scale);
-          f = 1.f;
+          for (int e = 0; e < 4 * NB; e++)
+            s[rb][e >> 2][e & 3] = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s[rb][e >> 2][e & 3] * q_scale[rb]));
+          slope[rb] = 2.f * p.cap_log2e;
+          offset[rb] = p.cap_log2e;
         }
-        float top;
         if constexpr (MASKED) {
 #pragma unroll
           for (int h = 0; h < NB / 2; h++) seen_bits[rb][h] = 0;
 #pragma unroll
           for (int e = 0; e < 4 * NB; e++) {
             const bool seen = tok + 16 * (e >> 2) + 4 * g + (e & 3) < limit[rb];
-            s[rb][e >> 2][e & 3] = seen ? s[rb][e >> 2][e & 3] * f : -INFINITY;
+            s[rb][e >> 2][e & 3] = seen ? __builtin_fmaf(s[rb][e >> 2][e & 3], slope[rb], offset[rb]) : -INFINITY;
             seen_bits[rb][e >> 3] |= seen ? 1u << (e & 7) : 0u;
           }
-          f = 1.f;
+          slope[rb] = 1.f;
+          offset[rb] = 0.f;
         }
         // (med3 with +inf is a maximum that the compiler schedules behind the matrix results, without quieting its operands first)
-        top = __builtin_amdgcn_fmed3f(s[rb][0][0], s[rb][0][1], INFINITY);
+        top[rb] = __builtin_amdgcn_fmed3f(s[rb][0][0], s[rb][0][1], INFINITY);
 #pragma unroll
-        for (int e = 2; e < 4 * NB; e++) top = __builtin_amdgcn_fmed3f(top, s[rb][e >> 2][e & 3], INFINITY);
-        top = group_max(top) * f;  // (f >= 0: the sign of the softmax scale is in the query)
-        if (__ballot(top > m_run[rb] + kRescaleGap4)) {  // (the first tile with a visible token always comes here)
-          const float m_new = top > m_run[rb] + kRescaleGap4 ? top : m_run[rb];
+        for (int e = 2; e < 4 * NB; e++) top[rb] = __builtin_amdgcn_fmed3f(top[rb], s[rb][e >> 2][e & 3], INFINITY);
+        top[rb] = __builtin_fmaf(group_max(top[rb]), slope[rb], offset[rb]);
+        grown |= top[rb] > m_run[rb] + kRescaleGap4;
+      }
+      if (__ballot(grown)) {  // (the first tile with a visible token always comes here)
+#pragma unroll
+        for (int rb = 0; rb < NRB; rb++) {
+          const float m_new = top[rb] > m_run[rb] + kRescaleGap4 ? top[rb] : m_run[rb];
           const float shrink = fast_exp2(m_run[rb] - m_new);
           m_run[rb] = m_new;
           lsum[rb] *= shrink;
 #pragma unroll
           for (int n = 0; n < DPL; n++) o[rb][n] *= shrink;
         }
+      }
+#pragma unroll
+      for (int rb = 0; rb < NRB; rb++) {
+        const float shift = offset[rb] - m_run[rb];
 #pragma unroll
         for (int h = 0; h < NB / 2; h++) {
           float pr[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) pr[e] = fast_exp2(__builtin_fmaf(s[rb][2 * h + (e >> 2)][e & 3], f, -m_run[rb]));
+          for (int e = 0; e < 8; e++) pr[e] = fast_exp2(__builtin_fmaf(s[rb][2 * h + (e >> 2)][e & 3], slope[rb], shift));
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             pw[rb][h][0][e] = pack_bf16(pr[2 * e], pr[2 * e + 1]);
@@ -639,68 +654,96 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   }
 }
 
-// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  One wave per row, a
-// lane has four head elements, so the 64 / (D / 4) lane groups of a wave take different ranges; eight loads of each group are in
-// flight before the first weight is known.  Sequences without tokens get zeros here.
-template <typename QT, int D>
+// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  One wave takes R rows
+// (four where there are tens of thousands, so that they are one round of waves); a lane has four head elements, so the 64 / (D / 4)
+// lane groups of a wave take different ranges.  All rows' first loads are in flight before the first weight is known.  Sequences
+// without tokens get zeros here.
+template <typename QT, int D, int R, int PRE>
+__device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t row0, int64_t rows_all, int first, int n, bool second) {
+  constexpr int LPR = D / 4, GROUPS = 64 / LPR;  // lanes per row, ranges side by side; PRE: loads of a row in flight
+  const int lane = threadIdx.x & 63, grp = lane / LPR, d0 = 4 * (lane % LPR);
+  auto slot_of = [&](int i, int64_t row) __attribute__((always_inline)) -> int64_t {
+    const int k = min(i, n - 1);
+    return (int64_t)(2 * (first + k) + (k == 0 && second ? 1 : 0)) * rows_all + row;
+  };
+  f32x4 acc[R];
+  float M[R], W[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    M[r] = -INFINITY;
+    W[r] = 0.f;
+  }
+  for (int base = 0; base < n; base += PRE * GROUPS) {
+    f32x4 x[R][PRE];
+    float lse[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int64_t row = row0 + r < rows_all ? row0 + r : rows_all - 1;
+#pragma unroll
+      for (int i = 0; i < PRE; i++) x[r][i] = *(const f32x4*)(p.part_o + slot_of(base + i * GROUPS + grp, row) * D + d0);
+      lse[r] = lane < PRE * GROUPS && base + lane < n ? p.part_lse[slot_of(base + lane, row)] : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float top = lse[r];
+#pragma unroll
+      for (int m = 1; m < PRE * GROUPS; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+      top = fmaxf(M[r], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, top), 0)));
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float shrink = fast_exp2(M[r] - ref), wl = fast_exp2(lse[r] - ref);  // (NaN stays NaN)
+      M[r] = top;
+      W[r] *= shrink;
+      acc[r] *= shrink;
+#pragma unroll
+      for (int i = 0; i < PRE; i++) {
+        const float w = __shfl(wl, i * GROUPS + grp, 64);
+        W[r] += w;
+        if (w != 0.f) acc[r] += w * x[r][i];  // (a place past the last has no weight)
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+#pragma unroll
+    for (int m = LPR; m < 64; m <<= 1) {
+      W[r] += __shfl_xor(W[r], m, 64);
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[r][e] += __shfl_xor(acc[r][e], m, 64);
+    }
+    const int64_t row = row0 + r;
+    if (grp > 0 || row >= rows_all) continue;
+    const float inv = W[r] == 0.f ? 0.f : 1.0f / W[r];
+    const int kvh = (int)(row / p.rows), qr = (int)(row - (int64_t)kvh * p.rows), s = qr / p.group, gi = qr - s * p.group;
+    *(u32x2*)(p.out + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D + d0) =
+        u32x2{pack16<QT>(acc[r][0] * inv, acc[r][1] * inv), pack16<QT>(acc[r][2] * inv, acc[r][3] * inv)};
+  }
+}
+
+template <typename QT, int D, int R>
 __global__ __launch_bounds__(256) void paged_decode_fp4_merge_kernel(const Fp4Params p) {
-  constexpr int LPR = D / 4, GROUPS = 64 / LPR, PRE = 8;  // lanes per row, ranges side by side, loads in flight
-  const int lane = threadIdx.x & 63, b = blockIdx.y, grp = lane / LPR, d0 = 4 * (lane % LPR);
-  const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
-  const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
+  const int b = blockIdx.y;
+  const int64_t rows_all = (int64_t)p.heads_kv * p.rows, row0 = ((int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6)) * R;
   int pre;
   const int T = total_units(p, b, &pre);
   const int nu = uni(units_of_len(len_of(p, b)));
   int first = 0, last = -1;
   bool second = false;
-  const Ranges ranges(T, p.n_parts);
   if (nu > 0) {
+    const Ranges ranges(T, p.n_parts);
     first = uni(ranges.owner(pre));
     last = uni(ranges.owner(pre + nu - 1));
     if (first == last) return;  // written by the range that holds it
     second = ranges.begin(first) != pre;
   }
-  if (row >= rows_all) return;
+  if (row0 >= rows_all) return;
   const int n = last - first + 1;
-  auto slot_of = [&](int i) __attribute__((always_inline)) -> int64_t {
-    const int part = first + min(i, n - 1);
-    return (int64_t)(2 * part + (part == first && second ? 1 : 0)) * rows_all + row;
-  };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float M = -INFINITY, W = 0.f;
-  for (int base = 0; base < n; base += PRE * GROUPS) {
-    f32x4 x[PRE];
-#pragma unroll
-    for (int i = 0; i < PRE; i++) x[i] = *(const f32x4*)(p.part_o + slot_of(base + i * GROUPS + grp) * D + d0);
-    const bool there = lane < PRE * GROUPS && base + lane < n;
-    const float lse = there ? p.part_lse[slot_of(base + lane)] : -INFINITY;
-    float top = lse;
-#pragma unroll
-    for (int m = 1; m < PRE * GROUPS; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    top = fmaxf(M, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, top), 0)));
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float shrink = fast_exp2(M - ref), wl = fast_exp2(lse - ref);  // (NaN stays NaN)
-    M = top;
-    W *= shrink;
-    acc *= shrink;
-#pragma unroll
-    for (int i = 0; i < PRE; i++) {
-      const float w = __shfl(wl, i * GROUPS + grp, 64);
-      W += w;
-      if (w != 0.f) acc += w * x[i];  // (a row that saw nothing holds zeros, and a place past the last is not added)
-    }
+  constexpr int GROUPS = 256 / D;
+  if (n <= 2 * GROUPS) {
+    merge_rows<QT, D, R, 2>(p, b, row0, rows_all, first, n, second);
+  } else {
+    for (int r = 0; r < R && row0 + r < rows_all; r++) merge_rows<QT, D, 1, 8>(p, b, row0 + r, rows_all, first, n, second);
   }
-#pragma unroll
-  for (int m = LPR; m < 64; m <<= 1) {
-    W += __shfl_xor(W, m, 64);
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], m, 64);
-  }
-  if (grp > 0) return;
-  const float inv = W == 0.f ? 0.f : 1.0f / W;
-  const int kvh = (int)(row / p.rows), r = (int)(row - (int64_t)kvh * p.rows), s = r / p.group, gi = r - s * p.group;
-  *(u32x2*)(p.out + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D + d0) =
-      u32x2{pack16<QT>(acc[0] * inv, acc[1] * inv), pack16<QT>(acc[2] * inv, acc[3] * inv)};
 }
 
 constexpr int kMaxParts4 = 4096;
@@ -722,7 +765,10 @@ const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return hipGetErrorString(e);
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
-  hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D>), dim3((unsigned)((rows_all + 3) / 4), p.batch), dim3(256), 0, s, p);
+  if (rows_all * p.batch <= 8192)
+    hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 1>), dim3((unsigned)((rows_all + 3) / 4), p.batch), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 4>), dim3((unsigned)((rows_all + 15) / 16), p.batch), dim3(256), 0, s, p);
   e = hipGetLastError();
   return e == hipSuccess ? nullptr : hipGetErrorString(e);
 }
@@ -784,9 +830,8 @@ const char* launch_decode_fp4(const void* q, const void* k, const void* v, const
   // the kernel takes maxima before it scales: the sign of the scale goes into the query
   p.negate_q = sm_scale < 0.f;
   sm_scale = fabsf(sm_scale);
-  p.score_scale = sm_scale * kLog2e;
+  p.score_scale = softcap > 0.f ? 2.f * kLog2e * (sm_scale / softcap) : sm_scale * kLog2e;
   p.cap_log2e = softcap * kLog2e;
-  p.inv_cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f;
   return q_dtype == MI355_DT_BF16 ? launch_fp4_dim<bf16_tag>(p, dim, s) : launch_fp4_dim<fp16_tag>(p, dim, s);
 }
 

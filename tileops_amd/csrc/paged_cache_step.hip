@@ -227,8 +227,8 @@ __device__ __forceinline__ float load_side(const void* p, int64_t i, int fp32) {
   return fp32 ? ((const float*)p)[i] : load_x<XT>((const uint16_t*)p + i);
 }
 
-// One head of one token per wave, a pair of neighbouring elements per lane (two pairs at head dim 256).  R: the type that the
-// norm and the rotation are formed in.
+// The general form, for rows that the vector form below does not take: one head of one token per wave, a pair of neighbouring
+// elements per lane (two pairs at head dim 256).  R: the type that the norm and the rotation are formed in.
 template <typename XT, typename R>
 __device__ __forceinline__ void norm_rotate_pair(const AppendParams& p, const uint16_t* x, const void* weight, int64_t tpos, int d, R rstd, float* out) {
   auto normed = [&](int e) -> R {
@@ -347,6 +347,222 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendPa
   }
 }
 
+// The vector form: a lane has sixteen consecutive elements of a row (two 16-byte loads), a wave 1024 / dim rows at a time, rows of
+// one kind (query, key, value) counted through all tokens so that few kv heads still fill the wave.  The other half of a rotated pair
+// lies rotary_dim / 32 lanes away: its raw elements come over as eight dwords, and the lane norms them itself.  The next rows are
+// requested before the present ones are worked on; tables are read again only when the token changes.
+// Takes: rotary_dim a multiple of 32 (interleaved: of 16), rows, tables and weights 16-byte aligned.
+// Bound: memory.
+struct RowSide {  // cos and sin (with the sign of the pair's half) of a lane's sixteen elements
+  float c[16], s[16];
+};
+
+template <typename XT>
+__device__ __forceinline__ void load_side16(const void* p, int64_t i, int fp32, float* out) {
+  if (fp32) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const f32x4 w = *(const f32x4*)((const float*)p + i + 4 * e);
+#pragma unroll
+      for (int j = 0; j < 4; j++) out[4 * e + j] = w[j];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const u32x4 w = *(const u32x4*)((const uint16_t*)p + i + 8 * e);
+      const uint32_t raw[4] = {w[0], w[1], w[2], w[3]};
+      Unpack<XT, 8>::run(raw, out + 8 * e);
+    }
+  }
+}
+
+template <typename XT, typename R>
+__device__ __forceinline__ void norm_rotate16(const AppendParams& p, const uint32_t* x, const uint32_t* other, bool weighted, const float* w,
+                                              const float* w_other, const RowSide& t, int lanes, float* y) {
+  float xf[16], of[16];
+  Unpack<XT, 8>::run(x, xf);
+  Unpack<XT, 8>::run(x + 4, xf + 8);
+  R rstd = 1;
+  if (weighted) {
+    R sum = 0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sum += (R)xf[e] * (R)xf[e];
+    for (int m = 1; m < lanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
+    rstd = (R)1 / sqrt(sum / (R)p.dim + (R)p.eps);
+  }
+  R own[16];
+#pragma unroll
+  for (int e = 0; e < 16; e++) own[e] = weighted ? (R)xf[e] * rstd * (R)w[e] : (R)xf[e];
+  if (p.rotary_dim == 0) {
+#pragma unroll
+    for (int e = 0; e < 16; e++) y[e] = (float)own[e];
+  } else if (p.interleaved) {
+#pragma unroll
+    for (int e = 0; e < 16; e++) y[e] = (float)(own[e] * (R)t.c[e] + own[e ^ 1] * (R)t.s[e]);
+  } else {
+    Unpack<XT, 8>::run(other, of);
+    Unpack<XT, 8>::run(other + 4, of + 8);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const R o = weighted ? (R)of[e] * rstd * (R)w_other[e] : (R)of[e];
+      y[e] = (float)(own[e] * (R)t.c[e] + o * (R)t.s[e]);
+    }
+  }
+}
+
+template <typename XT, int CACHE>
+__global__ __launch_bounds__(256) void qk_norm_rope_append_rows_kernel(const AppendParams p, int passes, int q_waves, int k_waves) {
+  const int lane = threadIdx.x & 63;
+  const int lanes = p.dim >> 4, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
+  int wave = blockIdx.x * 4 + uni(threadIdx.x >> 6);
+  const bool is_q = wave < q_waves, is_k = !is_q && wave < q_waves + k_waves;
+  wave -= is_q ? 0 : is_k ? q_waves : q_waves + k_waves;
+  const int heads = is_q ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^31: the launcher checks)
+  const uint16_t* base = is_q ? p.q : is_k ? p.k : p.v;
+  const int64_t stride = is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride;
+  const void* weight = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
+  const bool rotates = (is_q || is_k) && p.rotary_dim > 0;
+  const int half = p.rotary_dim >> 1;
+  // partner lane of the halves form: rows of lanes beyond the rotated elements keep theirs
+  const bool turned = rotates && 16 * j < p.rotary_dim, upper = 16 * j >= half;
+  const int mate = turned && !p.interleaved ? (upper ? j - half / 16 : j + half / 16) : j;
+  float w[16], w_other[16];
+  if (weight) {
+    load_side16<XT>(weight, 16 * j, p.weight_fp32, w);
+    load_side16<XT>(weight, 16 * mate, p.weight_fp32, w_other);
+  }
+  const int first = wave * passes * per_wave + lane / lanes;
+  if (wave * passes * per_wave >= rows) return;
+  auto row_ptr = [&](int r, int* token, int* head) __attribute__((always_inline)) -> const uint16_t* {
+    r = min(r, rows - 1);  // (past the end: the last row again, which is not stored)
+    *token = r / heads;
+    *head = r - *token * heads;
+    return base + *token * stride + (int64_t)*head * p.dim + 16 * j;
+  };
+  int token, head, token_of_side = -1;
+  const uint16_t* src = row_ptr(first, &token, &head);
+  u32x4 n0 = *(const u32x4*)src, n1 = *(const u32x4*)(src + 8);
+  RowSide side;
+  for (int i = 0; i < passes; i++) {
+    const int r = first + i * per_wave, t = token, h = head;
+    if (r - lane / lanes >= rows) break;  // the whole wave is past the end
+    const uint32_t x[8] = {n0[0], n0[1], n0[2], n0[3], n1[0], n1[1], n1[2], n1[3]};
+    if (i + 1 < passes) {
+      src = row_ptr(r + per_wave, &token, &head);
+      n0 = *(const u32x4*)src;
+      n1 = *(const u32x4*)(src + 8);
+    }
+    int64_t slot = 0;
+    if (!is_q) slot = p.slots[t];
+    if (rotates && __ballot(t != token_of_side)) {
+      token_of_side = t;
+      const int64_t tpos = min(max(p.positions[t], 0), p.max_position - 1);  // never outside the tables
+      if (!turned) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          side.c[e] = 1.f;
+          side.s[e] = 0.f;
+        }
+      } else if (p.interleaved) {
+        // sixteen elements are eight pairs: two loads of four (or one of eight) values
+        float c8[8], s8[8];
+        const int64_t at = tpos * half + 8 * j;
+        if (p.table_fp32) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const f32x4 a = *(const f32x4*)((const float*)p.cos_table + at + 4 * e), b = *(const f32x4*)((const float*)p.sin_table + at + 4 * e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              c8[4 * e + k] = a[k];
+              s8[4 * e + k] = b[k];
+            }
+          }
+        } else {
+          const u32x4 a = *(const u32x4*)((const uint16_t*)p.cos_table + at), b = *(const u32x4*)((const uint16_t*)p.sin_table + at);
+          const uint32_t ra[4] = {a[0], a[1], a[2], a[3]}, rb[4] = {b[0], b[1], b[2], b[3]};
+          Unpack<XT, 8>::run(ra, c8);
+          Unpack<XT, 8>::run(rb, s8);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          side.c[e] = c8[e >> 1];
+          side.s[e] = e & 1 ? s8[e >> 1] : -s8[e >> 1];
+        }
+      } else {
+        const int64_t at = tpos * half + 16 * j - (upper ? half : 0);
+        load_side16<XT>(p.cos_table, at, p.table_fp32, side.c);
+        load_side16<XT>(p.sin_table, at, p.table_fp32, side.s);
+#pragma unroll
+        for (int e = 0; e < 16; e++) side.s[e] = upper ? side.s[e] : -side.s[e];
+      }
+    }
+    float y[16];
+    if (is_q || is_k) {
+      uint32_t other[8];
+      if (rotates && !p.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) other[e] = (uint32_t)__shfl((int)x[e], lane - j + mate, 64);
+      }
+      // keys that become codes: in 64 bits, rounded to 32 once (see the general form)
+      if (is_k && CACHE != kCache16) norm_rotate16<XT, double>(p, x, other, weight != nullptr, w, w_other, side, lanes, y);
+      else norm_rotate16<XT, float>(p, x, other, weight != nullptr, w, w_other, side, lanes, y);
+    } else {
+      Unpack<XT, 8>::run(x, y);
+      Unpack<XT, 8>::run(x + 4, y + 8);
+    }
+    const bool store = r < rows && (is_q || (slot >= 0 && slot < p.n_tokens));
+    const int64_t token_row = slot * p.heads_kv + h;  // row of a token-major pool
+    if (is_q || CACHE == kCache16) {
+      uint16_t* dst = (is_q ? p.q_out + (int64_t)r * p.dim : (uint16_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim) + 16 * j;
+      u32x4 o0, o1;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        o0[e] = (uint32_t)f32_to_elem_bits<XT>(y[2 * e]) | ((uint32_t)f32_to_elem_bits<XT>(y[2 * e + 1]) << 16);
+        o1[e] = (uint32_t)f32_to_elem_bits<XT>(y[8 + 2 * e]) | ((uint32_t)f32_to_elem_bits<XT>(y[8 + 2 * e + 1]) << 16);
+      }
+      if (store) {
+        *(u32x4*)dst = o0;
+        *(u32x4*)(dst + 8) = o1;
+      }
+    } else if (CACHE == kCacheFp8) {
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(y[e]));
+      for (int m = 1; m < lanes; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
+      const float sc = fmaxf(amax, 1e-4f) / 448.0f;
+      u32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float z[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) z[k] = fminf(fmaxf(y[4 * e + k] / sc, -448.0f), 448.0f);
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+        o[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+      }
+      if (store) {
+        *(u32x4*)((uint8_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim + 16 * j) = o;
+        if (j == 0) ((float*)(is_k ? p.k_scale : p.v_scale))[token_row] = sc;
+      }
+    } else {
+      // two lanes hold a block
+      uint32_t amax = 0;
+#pragma unroll
+      for (int e = 0; e < 16; e++) amax = max(amax, abs_bits(y[e]));
+      amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1, 64));
+      const uint32_t byte = fp4_scale_byte(amax);
+      u32x2 o = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e >> 2] |= fp4_pack2(y[2 * e], y[2 * e + 1], byte) << (8 * (e & 3));
+      if (store) {
+        const uint32_t page = (uint32_t)slot / (uint32_t)p.page_size, off = (uint32_t)slot - page * (uint32_t)p.page_size;
+        const int64_t row = ((int64_t)page * p.heads_kv + h) * p.page_size + off;
+        *(u32x2*)((uint8_t*)(is_k ? p.k_cache : p.v_cache) + row * (p.dim >> 1) + 8 * j) = o;
+        if ((j & 1) == 0) ((uint8_t*)(is_k ? p.k_scale : p.v_scale))[row * (p.dim >> 5) + (j >> 1)] = (uint8_t)byte;
+      }
+    }
+  }
+}
+
 // --------------------------------------------------------------------------------------------- rows of the 4-bit cache
 // Eight elements per thread (four bytes of codes in, sixteen out).  Slots outside the pool give zeros.
 template <typename XT>
@@ -410,6 +626,14 @@ const char* launch_kv_release(const uint8_t* finished, const int32_t* seqlens, c
   return launched();
 }
 
+namespace {
+// Passes of a wave: one while that leaves a few waves per SIMD, four (with the next rows requested ahead) beyond.
+int append_passes(int tokens, int heads, int heads_kv, int per_wave) {
+  const int64_t passes = (int64_t)tokens * (heads + 2 * heads_kv) / per_wave;
+  return passes < 8192 ? 1 : 4;
+}
+}  // namespace
+
 const char* launch_qk_norm_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                                        const void* q_weight, const void* k_weight, int weight_dtype, const void* cos_table,
                                        const void* sin_table, int table_dtype, int64_t max_position, const int32_t* positions,
@@ -447,16 +671,28 @@ const char* launch_qk_norm_rope_append(const void* q, const void* k, const void*
   p.table_fp32 = table_dtype == MI355_DT_FP32;
   p.interleaved = interleaved;
   const int cache = cache_dtype == MI355_DT_FP4_E2M1 ? kCacheFp4 : cache_dtype == MI355_DT_FP8_E4M3FN ? kCacheFp8 : kCache16;
+  const bool bf16 = x_dtype == MI355_DT_BF16;
+  const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table | (uintptr_t)sin_table;
+  const int64_t most_rows = (int64_t)tokens * (heads > heads_kv ? heads : heads_kv);
+  if (rotary_dim % (interleaved ? 16 : 32) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 30)) {
+    const int per_wave = 1024 / dim;
+    const int passes = append_passes(tokens, heads, heads_kv, per_wave);
+    auto waves = [&](int h) { return (int)(((int64_t)tokens * h + (int64_t)per_wave * passes - 1) / ((int64_t)per_wave * passes)); };
+    const int q_waves = waves(heads), k_waves = waves(heads_kv);
+    const dim3 grid((q_waves + 2 * k_waves + 3) / 4), block(256);
+    auto kern = bf16 ? (cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<bf16_tag, kCacheFp4>
+                        : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<bf16_tag, kCacheFp8> : qk_norm_rope_append_rows_kernel<bf16_tag, kCache16>)
+                     : (cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<fp16_tag, kCacheFp4>
+                        : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<fp16_tag, kCacheFp8> : qk_norm_rope_append_rows_kernel<fp16_tag, kCache16>);
+    hipLaunchKernelGGL(kern, grid, block, 0, s, p, passes, q_waves, k_waves);
+    return launched();
+  }
   const dim3 grid(tokens, (heads + 2 * heads_kv + 3) / 4), block(256);
-#define MI355_LAUNCH_APPEND(XT)                                                                                      \
-  do {                                                                                                               \
-    if (cache == kCacheFp4) hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCacheFp4>), grid, block, 0, s, p);   \
-    else if (cache == kCacheFp8) hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCacheFp8>), grid, block, 0, s, p); \
-    else hipLaunchKernelGGL((qk_norm_rope_append_kernel<XT, kCache16>), grid, block, 0, s, p);                       \
-  } while (0)
-  if (x_dtype == MI355_DT_BF16) MI355_LAUNCH_APPEND(bf16_tag);
-  else MI355_LAUNCH_APPEND(fp16_tag);
-#undef MI355_LAUNCH_APPEND
+  auto kern = bf16 ? (cache == kCacheFp4 ? qk_norm_rope_append_kernel<bf16_tag, kCacheFp4>
+                      : cache == kCacheFp8 ? qk_norm_rope_append_kernel<bf16_tag, kCacheFp8> : qk_norm_rope_append_kernel<bf16_tag, kCache16>)
+                   : (cache == kCacheFp4 ? qk_norm_rope_append_kernel<fp16_tag, kCacheFp4>
+                      : cache == kCacheFp8 ? qk_norm_rope_append_kernel<fp16_tag, kCacheFp8> : qk_norm_rope_append_kernel<fp16_tag, kCache16>);
+  hipLaunchKernelGGL(kern, grid, block, 0, s, p);
   return launched();
 }
 

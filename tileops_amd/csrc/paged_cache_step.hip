@@ -186,13 +186,22 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
   return (uint32_t)(max(e, -126) + 127);
 }
 
-// Two elements -> one byte of codes (round to nearest, ties to the even code).  The scale is a power of two: dividing by it is exact.
-__device__ __forceinline__ uint32_t fp4_pack2(float a, float b, uint32_t scale_byte) {
-  const float lim = 0x1.8p127f;
-  a = fminf(fmaxf(a, -lim), lim);
-  b = fminf(fmaxf(b, -lim), lim);
-  const uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, __uint_as_float(scale_byte << 23), 0);
-  return scale_byte == 255u ? 0u : (w & 0xffu);
+// N pairs of elements -> N bytes of codes (round to nearest, ties to the even code), the first in the lowest byte.  The scale is a power of
+// two: dividing by it is exact.
+template <int N>
+__device__ __forceinline__ uint32_t fp4_pack(const float* x, uint32_t scale_byte) {
+  const float lim = 0x1.8p127f, scale = __uint_as_float(scale_byte << 23);
+  float c[2 * N];
+#pragma unroll
+  for (int e = 0; e < 2 * N; e++) c[e] = __builtin_amdgcn_fmed3f(x[e], -lim, lim);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[0], c[1], scale, 0);
+  if constexpr (N == 4) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[2], c[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[4], c[5], scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[6], c[7], scale, 3);
+  }
+  return scale_byte == 255u ? 0u : w;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -211,6 +220,7 @@ struct AppendParams {
   int tokens, heads, heads_kv, dim, rotary_dim, max_position, page_size;
   double eps;
   int weight_fp32, table_fp32, interleaved;
+  int page_shift;  // log2 of page_size, -1 if it is no power of two
 };
 
 enum { kCache16 = 0, kCacheFp8 = 1, kCacheFp4 = 2 };
@@ -342,224 +352,302 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendPa
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, m, 64));
     const uint32_t byte = fp4_scale_byte(amax);
-    codes[i] = (uint8_t)fp4_pack2(y[j][0], y[j][1], byte);
+    codes[i] = (uint8_t)fp4_pack<1>(y[j], byte);
     if ((lane & 15) == 0) scales[i >> 4] = (uint8_t)byte;
   }
 }
 
-// The vector form: a lane has sixteen consecutive elements of a row (two 16-byte loads), a wave 1024 / dim rows at a time, rows of
-// one kind (query, key, value) counted through all tokens so that few kv heads still fill the wave.  The other half of a rotated pair
-// lies rotary_dim / 32 lanes away: its raw elements come over as eight dwords, and the lane norms them itself.  The next rows are
-// requested before the present ones are worked on; tables are read again only when the token changes.
-// Takes: rotary_dim a multiple of 32 (interleaved: of 16), rows, tables and weights 16-byte aligned.
+// The vector form: a lane has eight consecutive elements of a row (16 bytes), a wave 512 / dim rows at a time, rows of one kind (query,
+// key, value) counted through all tokens so that few kv heads still fill the wave.  The other half of a rotated pair lies rotary_dim / 16
+// lanes away: its raw elements come over as four dwords, and the lane norms them itself.  The next rows are requested before the
+// present ones are worked on; tables are read again only when the token changes.
+// Takes: rotary_dim a multiple of 16 (interleaved: of 8), rows, tables and weights 16-byte aligned.
 // Bound: memory.
-struct RowSide {  // cos and sin (with the sign of the pair's half) of a lane's sixteen elements
-  float c[16], s[16];
+// Four values (16-bit or fp32) of a weight or table as floats.
+template <typename XT>
+__device__ __forceinline__ f32x4 load_side4(const void* p, int64_t i, int fp32) {
+  if (fp32) return *(const f32x4*)((const float*)p + i);
+  const u32x2 w = *(const u32x2*)((const uint16_t*)p + i);
+  const uint32_t raw[2] = {w[0], w[1]};
+  float out[4];
+  Unpack<XT, 4>::run(raw, out);
+  return f32x4{out[0], out[1], out[2], out[3]};
+}
+
+// Reductions over the 8, 16 or 32 neighbouring lanes of a row on the data-parallel-primitive path: lanes one and two apart, then
+// (groups of four being equal) the mirrored half row and the mirrored row, then the neighbouring row of sixteen.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ float dpp(float x) { return __uint_as_float(dpp<CTRL>(__float_as_uint(x))); }
+template <int CTRL> __device__ __forceinline__ double dpp(double x) {
+  const u32x2 w = __builtin_bit_cast(u32x2, x);
+  return __builtin_bit_cast(double, u32x2{dpp<CTRL>(w[0]), dpp<CTRL>(w[1])});
+}
+__device__ __forceinline__ uint32_t other_row(uint32_t x) {  // the same lane of the other row of sixteen in a pair of rows
+  const u32x2 r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return (threadIdx.x & 16) ? r[0] : r[1];
+}
+__device__ __forceinline__ float other_row(float x) { return __uint_as_float(other_row(__float_as_uint(x))); }
+__device__ __forceinline__ double other_row(double x) {
+  const u32x2 w = __builtin_bit_cast(u32x2, x);
+  return __builtin_bit_cast(double, u32x2{other_row(w[0]), other_row(w[1])});
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+template <typename T, typename F>
+__device__ __forceinline__ T over_row(T x, int lanes, F f) {
+  x = f(x, dpp<kXor1>(x));
+  x = f(x, dpp<kXor2>(x));
+  x = f(x, dpp<kHalfMirror>(x));
+  if (lanes > 8) x = f(x, dpp<kMirror>(x));
+  if (lanes > 16) x = f(x, other_row(x));
+  return x;
+}
+
+__device__ __forceinline__ float inverse_root(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inverse_root(double x) {  // the hardware's estimate and two Newton steps
+  double r = __builtin_amdgcn_rsq(x);
+  if (!(r > 0.0 && r < __builtin_inf())) return r;
+  r = r * (1.5 - 0.5 * x * r * r);
+  return r * (1.5 - 0.5 * x * r * r);
+}
+
+// Where a lane's eight elements stand in the rotation.
+struct Turn {
+  bool on, upper;  // they are rotated; they are the second half of their pairs
+  int mate;        // lane of the row that holds the other half (its own if interleaved or not rotated)
+};
+
+// Coefficients of elements 4k .. 4k + 3 of the lane: y[e] = own[e] * c[e] + other[e] * s[e] with own, other normed rows.
+template <typename XT>
+__device__ __forceinline__ void side4(const AppendParams& p, const Turn& t, int64_t tpos, int j, int k, f32x4* c, f32x4* s) {
+  const int half = p.rotary_dim >> 1;
+  if (!t.on) {
+    *c = f32x4{1.f, 1.f, 1.f, 1.f};
+    *s = f32x4{0.f, 0.f, 0.f, 0.f};
+  } else if (p.interleaved) {
+    const int64_t at = tpos * half + 4 * j + 2 * k;
+    float c0, c1, s0, s1;
+    if (p.table_fp32) {
+      const f32x2 a = *(const f32x2*)((const float*)p.cos_table + at), b = *(const f32x2*)((const float*)p.sin_table + at);
+      c0 = a[0], c1 = a[1], s0 = b[0], s1 = b[1];
+    } else {
+      const uint32_t ra[1] = {*(const uint32_t*)((const uint16_t*)p.cos_table + at)}, rb[1] = {*(const uint32_t*)((const uint16_t*)p.sin_table + at)};
+      float a[2], b[2];
+      Unpack<XT, 2>::run(ra, a);
+      Unpack<XT, 2>::run(rb, b);
+      c0 = a[0], c1 = a[1], s0 = b[0], s1 = b[1];
+    }
+    *c = f32x4{c0, c0, c1, c1};
+    *s = f32x4{-s0, s0, -s1, s1};
+  } else {
+    const int64_t at = tpos * half + 8 * j - (t.upper ? half : 0) + 4 * k;
+    *c = load_side4<XT>(p.cos_table, at, p.table_fp32);
+    *s = load_side4<XT>(p.sin_table, at, p.table_fp32);
+    if (!t.upper) *s = -*s;
+  }
+}
+
+// x / s for many values and one s in [2^-23, 2^120], |x| <= 448 s: the quotient corrected once by its remainder (Markstein), with one
+// reciprocal for all of them instead of one division each.
+struct Quotient {
+  float s, r;
+  __device__ __forceinline__ explicit Quotient(float d) : s(d) {
+    const float r0 = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(__builtin_fmaf(-d, r0, 1.0f), r0, r0);
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = x * r;
+    return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-s, q, x), r, q), x);  // (a zero keeps its sign)
+  }
 };
 
 template <typename XT>
-__device__ __forceinline__ void load_side16(const void* p, int64_t i, int fp32, float* out) {
-  if (fp32) {
+__device__ __forceinline__ u32x4 pack_row8(const float* y) {
+  u32x4 o;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const f32x4 w = *(const f32x4*)((const float*)p + i + 4 * e);
+  for (int e = 0; e < 4; e++) o[e] = (uint32_t)f32_to_elem_bits<XT>(y[2 * e]) | ((uint32_t)f32_to_elem_bits<XT>(y[2 * e + 1]) << 16);
+  return o;
+}
+
+// Eight finished elements of row (token, head h) of a kind into the cache.
+template <typename XT, int CACHE>
+__device__ __forceinline__ void store_cached(const AppendParams& p, void* cache, void* scale, const float* y, int64_t slot, int h, int lanes, int j, bool store) {
+  const int64_t token_row = slot * p.heads_kv + h;  // row of a token-major pool
+  if constexpr (CACHE == kCache16) {
+    if (store) *(u32x4*)((uint16_t*)cache + token_row * p.dim + 8 * j) = pack_row8<XT>(y);
+  } else if constexpr (CACHE == kCacheFp8) {
+    float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; j++) out[4 * e + j] = w[j];
-    }
-  } else {
+    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(y[e]));
+    amax = over_row(amax, lanes, [](float a, float b) { return fmaxf(a, b); });
+    const float sc = fmaxf(amax, 1e-4f) / 448.0f;
+    const Quotient over(sc);
+    const bool plain = sc < 0x1p100f;  // (else an infinity or close to one: the division itself)
+    u32x2 o;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const u32x4 w = *(const u32x4*)((const uint16_t*)p + i + 8 * e);
-      const uint32_t raw[4] = {w[0], w[1], w[2], w[3]};
-      Unpack<XT, 8>::run(raw, out + 8 * e);
+      float z[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float v = y[4 * e + k];
+        z[k] = fminf(fmaxf(plain ? over(v) : v / sc, -448.0f), 448.0f);
+      }
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+      o[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+    }
+    if (store) {
+      *(u32x2*)((uint8_t*)cache + token_row * p.dim + 8 * j) = o;
+      if (j == 0) ((float*)scale)[token_row] = sc;
+    }
+  } else {
+    // four lanes hold a block
+    uint32_t amax = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) amax = max(amax, abs_bits(y[e]));
+    amax = max(amax, dpp<kXor1>(amax));
+    amax = max(amax, dpp<kXor2>(amax));
+    const uint32_t byte = fp4_scale_byte(amax);
+    const uint32_t o = fp4_pack<4>(y, byte);
+    if (store) {
+      const uint32_t page = p.page_shift >= 0 ? (uint32_t)slot >> p.page_shift : (uint32_t)slot / (uint32_t)p.page_size;
+      const uint32_t off = (uint32_t)slot - page * (uint32_t)p.page_size;
+      const int64_t row = ((int64_t)page * p.heads_kv + h) * p.page_size + off;
+      *(uint32_t*)((uint8_t*)cache + row * (p.dim >> 1) + 4 * j) = o;
+      if ((j & 3) == 0) ((uint8_t*)scale)[row * (p.dim >> 5) + (j >> 2)] = (uint8_t)byte;
     }
   }
 }
 
-template <typename XT, typename R>
-__device__ __forceinline__ void norm_rotate16(const AppendParams& p, const uint32_t* x, const uint32_t* other, bool weighted, const float* w,
-                                              const float* w_other, const RowSide& t, int lanes, float* y) {
-  float xf[16], of[16];
-  Unpack<XT, 8>::run(x, xf);
-  Unpack<XT, 8>::run(x + 4, xf + 8);
-  R rstd = 1;
-  if (weighted) {
-    R sum = 0;
+enum { kQuery, kKey, kValue };
+
+// Rows of one kind.  R: the type that norm and rotation are formed in (see the general form).
+template <typename XT, int CACHE, int KIND, typename R>
+__device__ __forceinline__ void append_rows(const AppendParams& p, int wave, int passes) {
+  const int lane = threadIdx.x & 63;
+  const int lanes = p.dim >> 3, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
+  const int heads = KIND == kQuery ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^30: the launcher checks)
+  const int row0 = wave * passes * per_wave;
+  if (row0 >= rows) return;
+  const uint16_t* base = KIND == kQuery ? p.q : KIND == kKey ? p.k : p.v;
+  const int64_t stride = KIND == kQuery ? p.q_stride : KIND == kKey ? p.k_stride : p.v_stride;
+  const void* weight = KIND == kQuery ? p.q_weight : KIND == kKey ? p.k_weight : nullptr;
+  const bool rotates = KIND != kValue && p.rotary_dim > 0;
+  const int apart = p.rotary_dim >> 4;  // lanes between the halves of a pair
+  Turn turn;
+  turn.on = rotates && 8 * j < p.rotary_dim;
+  turn.upper = j >= apart;
+  turn.mate = turn.on && !p.interleaved ? (turn.upper ? j - apart : j + apart) : j;
+  const int mate_lane = lane - j + turn.mate;
+
+  // the lane's row of the pass that is requested next: token and head, stepped instead of divided
+  const int dt = per_wave / heads, dh = per_wave - dt * heads;
+  int token = (row0 + lane / lanes) / heads, head = row0 + lane / lanes - token * heads;
+  const R inv_dim = (R)1 / (R)p.dim;  // (a power of two)
+  auto request = [&]() __attribute__((always_inline)) -> u32x4 {
+    const int t = min(token, p.tokens - 1);  // (past the end: a row of the last token again, which is not stored)
+    return *(const u32x4*)(base + t * stride + head * p.dim + 8 * j);
+  };
+  u32x4 ahead = request();
+  int token_of_side = -1;
+  f32x4 wc[2], ws[2];  // weight times cosine, the other half's weight times sine
+  for (int i = 0; i < passes; i++) {
+    if (row0 + i * per_wave >= rows) break;
+    const int r = row0 + i * per_wave + lane / lanes, t = min(token, p.tokens - 1), h = head;
+    const uint32_t x[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
+    token += dt;
+    head += dh;
+    if (head >= heads) {
+      head -= heads;
+      token++;
+    }
+    if (i + 1 < passes) ahead = request();
+    int64_t slot = 0;
+    if constexpr (KIND != kQuery) slot = p.slots[t];
+    float y[8];
+    if constexpr (KIND == kValue) {
+      Unpack<XT, 8>::run(x, y);
+    } else {
+      int64_t tpos = 0;
+      if (rotates) tpos = min(max(p.positions[t], 0), p.max_position - 1);  // never outside the tables
+      uint32_t other[4];
+      if (rotates) {
+        if (p.interleaved) {
 #pragma unroll
-    for (int e = 0; e < 16; e++) sum += (R)xf[e] * (R)xf[e];
-    for (int m = 1; m < lanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
-    rstd = (R)1 / sqrt(sum / (R)p.dim + (R)p.eps);
-  }
-  R own[16];
+          for (int e = 0; e < 4; e++) other[e] = __builtin_amdgcn_alignbit(x[e], x[e], 16);  // the pair's elements changed over
+        } else {
 #pragma unroll
-  for (int e = 0; e < 16; e++) own[e] = weighted ? (R)xf[e] * rstd * (R)w[e] : (R)xf[e];
-  if (p.rotary_dim == 0) {
+          for (int e = 0; e < 4; e++) other[e] = (uint32_t)__shfl((int)x[e], mate_lane, 64);
+        }
+      }
+      float xf[8];
+      Unpack<XT, 8>::run(x, xf);
+      R rstd = 1;
+      if (weight) {
+        R sum = 0;
 #pragma unroll
-    for (int e = 0; e < 16; e++) y[e] = (float)own[e];
-  } else if (p.interleaved) {
+        for (int e = 0; e < 8; e++) sum += (R)xf[e] * (R)xf[e];
+        sum = over_row(sum, lanes, [](R a, R b) { return a + b; });
+        rstd = inverse_root(sum * inv_dim + (R)p.eps);
+      }
+      if constexpr (sizeof(R) == 4) {
+        if (i == 0 || (rotates && __ballot(t != token_of_side))) {
+          token_of_side = t;
 #pragma unroll
-    for (int e = 0; e < 16; e++) y[e] = (float)(own[e] * (R)t.c[e] + own[e ^ 1] * (R)t.s[e]);
-  } else {
-    Unpack<XT, 8>::run(other, of);
-    Unpack<XT, 8>::run(other + 4, of + 8);
+          for (int k = 0; k < 2; k++) {
+            side4<XT>(p, turn, tpos, j, k, &wc[k], &ws[k]);
+            if (weight) {
+              const f32x4 w = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32), wo = load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
+              wc[k] *= w;
+              ws[k] *= p.interleaved ? f32x4{w[1], w[0], w[3], w[2]} : wo;
+            }
+          }
+        }
+        float of[8];
+        if (rotates) Unpack<XT, 8>::run(other, of);
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const R o = weighted ? (R)of[e] * rstd * (R)w_other[e] : (R)of[e];
-      y[e] = (float)(own[e] * (R)t.c[e] + o * (R)t.s[e]);
+        for (int e = 0; e < 8; e++) {
+          float z = xf[e] * wc[e >> 2][e & 3];
+          if (rotates) z = __builtin_fmaf(of[e], ws[e >> 2][e & 3], z);
+          y[e] = z * rstd;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          f32x4 c, s, w = {1.f, 1.f, 1.f, 1.f}, wo = w;
+          side4<XT>(p, turn, tpos, j, k, &c, &s);
+          if (weight) {
+            w = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32);
+            wo = p.interleaved ? f32x4{w[1], w[0], w[3], w[2]} : load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
+          }
+          float of[4] = {0.f, 0.f, 0.f, 0.f};
+          if (rotates) Unpack<XT, 4>::run(other + 2 * k, of);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            R z = (R)xf[4 * k + e] * (R)w[e] * (R)c[e];
+            if (rotates) z += (R)of[e] * (R)wo[e] * (R)s[e];
+            y[4 * k + e] = (float)(z * rstd);
+          }
+        }
+      }
+    }
+    const bool store = r < rows && (KIND == kQuery || (slot >= 0 && slot < p.n_tokens));
+    if constexpr (KIND == kQuery) {
+      if (store) *(u32x4*)(p.q_out + (int64_t)r * p.dim + 8 * j) = pack_row8<XT>(y);
+    } else {
+      store_cached<XT, CACHE>(p, KIND == kKey ? p.k_cache : p.v_cache, KIND == kKey ? p.k_scale : p.v_scale, y, slot, h, lanes, j, store);
     }
   }
 }
 
 template <typename XT, int CACHE>
-__global__ __launch_bounds__(256) void qk_norm_rope_append_rows_kernel(const AppendParams p, int passes, int q_waves, int k_waves) {
-  const int lane = threadIdx.x & 63;
-  const int lanes = p.dim >> 4, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
+__global__ __launch_bounds__(256, 4) void qk_norm_rope_append_rows_kernel(const AppendParams p, int passes, int q_waves, int k_waves) {
   int wave = blockIdx.x * 4 + uni(threadIdx.x >> 6);
-  const bool is_q = wave < q_waves, is_k = !is_q && wave < q_waves + k_waves;
-  wave -= is_q ? 0 : is_k ? q_waves : q_waves + k_waves;
-  const int heads = is_q ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^31: the launcher checks)
-  const uint16_t* base = is_q ? p.q : is_k ? p.k : p.v;
-  const int64_t stride = is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride;
-  const void* weight = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-  const bool rotates = (is_q || is_k) && p.rotary_dim > 0;
-  const int half = p.rotary_dim >> 1;
-  // partner lane of the halves form: rows of lanes beyond the rotated elements keep theirs
-  const bool turned = rotates && 16 * j < p.rotary_dim, upper = 16 * j >= half;
-  const int mate = turned && !p.interleaved ? (upper ? j - half / 16 : j + half / 16) : j;
-  float w[16], w_other[16];
-  if (weight) {
-    load_side16<XT>(weight, 16 * j, p.weight_fp32, w);
-    load_side16<XT>(weight, 16 * mate, p.weight_fp32, w_other);
-  }
-  const int first = wave * passes * per_wave + lane / lanes;
-  if (wave * passes * per_wave >= rows) return;
-  auto row_ptr = [&](int r, int* token, int* head) __attribute__((always_inline)) -> const uint16_t* {
-    r = min(r, rows - 1);  // (past the end: the last row again, which is not stored)
-    *token = r / heads;
-    *head = r - *token * heads;
-    return base + *token * stride + (int64_t)*head * p.dim + 16 * j;
-  };
-  int token, head, token_of_side = -1;
-  const uint16_t* src = row_ptr(first, &token, &head);
-  u32x4 n0 = *(const u32x4*)src, n1 = *(const u32x4*)(src + 8);
-  RowSide side;
-  for (int i = 0; i < passes; i++) {
-    const int r = first + i * per_wave, t = token, h = head;
-    if (r - lane / lanes >= rows) break;  // the whole wave is past the end
-    const uint32_t x[8] = {n0[0], n0[1], n0[2], n0[3], n1[0], n1[1], n1[2], n1[3]};
-    if (i + 1 < passes) {
-      src = row_ptr(r + per_wave, &token, &head);
-      n0 = *(const u32x4*)src;
-      n1 = *(const u32x4*)(src + 8);
-    }
-    int64_t slot = 0;
-    if (!is_q) slot = p.slots[t];
-    if (rotates && __ballot(t != token_of_side)) {
-      token_of_side = t;
-      const int64_t tpos = min(max(p.positions[t], 0), p.max_position - 1);  // never outside the tables
-      if (!turned) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          side.c[e] = 1.f;
-          side.s[e] = 0.f;
-        }
-      } else if (p.interleaved) {
-        // sixteen elements are eight pairs: two loads of four (or one of eight) values
-        float c8[8], s8[8];
-        const int64_t at = tpos * half + 8 * j;
-        if (p.table_fp32) {
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const f32x4 a = *(const f32x4*)((const float*)p.cos_table + at + 4 * e), b = *(const f32x4*)((const float*)p.sin_table + at + 4 * e);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              c8[4 * e + k] = a[k];
-              s8[4 * e + k] = b[k];
-            }
-          }
-        } else {
-          const u32x4 a = *(const u32x4*)((const uint16_t*)p.cos_table + at), b = *(const u32x4*)((const uint16_t*)p.sin_table + at);
-          const uint32_t ra[4] = {a[0], a[1], a[2], a[3]}, rb[4] = {b[0], b[1], b[2], b[3]};
-          Unpack<XT, 8>::run(ra, c8);
-          Unpack<XT, 8>::run(rb, s8);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          side.c[e] = c8[e >> 1];
-          side.s[e] = e & 1 ? s8[e >> 1] : -s8[e >> 1];
-        }
-      } else {
-        const int64_t at = tpos * half + 16 * j - (upper ? half : 0);
-        load_side16<XT>(p.cos_table, at, p.table_fp32, side.c);
-        load_side16<XT>(p.sin_table, at, p.table_fp32, side.s);
-#pragma unroll
-        for (int e = 0; e < 16; e++) side.s[e] = upper ? side.s[e] : -side.s[e];
-      }
-    }
-    float y[16];
-    if (is_q || is_k) {
-      uint32_t other[8];
-      if (rotates && !p.interleaved) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) other[e] = (uint32_t)__shfl((int)x[e], lane - j + mate, 64);
-      }
-      // keys that become codes: in 64 bits, rounded to 32 once (see the general form)
-      if (is_k && CACHE != kCache16) norm_rotate16<XT, double>(p, x, other, weight != nullptr, w, w_other, side, lanes, y);
-      else norm_rotate16<XT, float>(p, x, other, weight != nullptr, w, w_other, side, lanes, y);
-    } else {
-      Unpack<XT, 8>::run(x, y);
-      Unpack<XT, 8>::run(x + 4, y + 8);
-    }
-    const bool store = r < rows && (is_q || (slot >= 0 && slot < p.n_tokens));
-    const int64_t token_row = slot * p.heads_kv + h;  // row of a token-major pool
-    if (is_q || CACHE == kCache16) {
-      uint16_t* dst = (is_q ? p.q_out + (int64_t)r * p.dim : (uint16_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim) + 16 * j;
-      u32x4 o0, o1;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        o0[e] = (uint32_t)f32_to_elem_bits<XT>(y[2 * e]) | ((uint32_t)f32_to_elem_bits<XT>(y[2 * e + 1]) << 16);
-        o1[e] = (uint32_t)f32_to_elem_bits<XT>(y[8 + 2 * e]) | ((uint32_t)f32_to_elem_bits<XT>(y[8 + 2 * e + 1]) << 16);
-      }
-      if (store) {
-        *(u32x4*)dst = o0;
-        *(u32x4*)(dst + 8) = o1;
-      }
-    } else if (CACHE == kCacheFp8) {
-      float amax = 0.f;
-#pragma unroll
-      for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(y[e]));
-      for (int m = 1; m < lanes; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
-      const float sc = fmaxf(amax, 1e-4f) / 448.0f;
-      u32x4 o;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float z[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) z[k] = fminf(fmaxf(y[4 * e + k] / sc, -448.0f), 448.0f);
-        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-        o[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
-      }
-      if (store) {
-        *(u32x4*)((uint8_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim + 16 * j) = o;
-        if (j == 0) ((float*)(is_k ? p.k_scale : p.v_scale))[token_row] = sc;
-      }
-    } else {
-      // two lanes hold a block
-      uint32_t amax = 0;
-#pragma unroll
-      for (int e = 0; e < 16; e++) amax = max(amax, abs_bits(y[e]));
-      amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1, 64));
-      const uint32_t byte = fp4_scale_byte(amax);
-      u32x2 o = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; e++) o[e >> 2] |= fp4_pack2(y[2 * e], y[2 * e + 1], byte) << (8 * (e & 3));
-      if (store) {
-        const uint32_t page = (uint32_t)slot / (uint32_t)p.page_size, off = (uint32_t)slot - page * (uint32_t)p.page_size;
-        const int64_t row = ((int64_t)page * p.heads_kv + h) * p.page_size + off;
-        *(u32x2*)((uint8_t*)(is_k ? p.k_cache : p.v_cache) + row * (p.dim >> 1) + 8 * j) = o;
-        if ((j & 1) == 0) ((uint8_t*)(is_k ? p.k_scale : p.v_scale))[row * (p.dim >> 5) + (j >> 1)] = (uint8_t)byte;
-      }
-    }
+  if (wave < k_waves) {  // (the longest rows first)
+    if constexpr (CACHE == kCache16) append_rows<XT, CACHE, kKey, float>(p, wave, passes);
+    else append_rows<XT, CACHE, kKey, double>(p, wave, passes);
+  } else if ((wave -= k_waves) < q_waves) {
+    append_rows<XT, CACHE, kQuery, float>(p, wave, passes);
+  } else {
+    append_rows<XT, CACHE, kValue, float>(p, wave - q_waves, passes);
   }
 }
 
@@ -670,12 +758,13 @@ const char* launch_qk_norm_rope_append(const void* q, const void* k, const void*
   p.weight_fp32 = weight_dtype == MI355_DT_FP32;
   p.table_fp32 = table_dtype == MI355_DT_FP32;
   p.interleaved = interleaved;
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   const int cache = cache_dtype == MI355_DT_FP4_E2M1 ? kCacheFp4 : cache_dtype == MI355_DT_FP8_E4M3FN ? kCacheFp8 : kCache16;
   const bool bf16 = x_dtype == MI355_DT_BF16;
   const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table | (uintptr_t)sin_table;
   const int64_t most_rows = (int64_t)tokens * (heads > heads_kv ? heads : heads_kv);
-  if (rotary_dim % (interleaved ? 16 : 32) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 30)) {
-    const int per_wave = 1024 / dim;
+  if (rotary_dim % (interleaved ? 8 : 16) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 30)) {
+    const int per_wave = 512 / dim;
     const int passes = append_passes(tokens, heads, heads_kv, per_wave);
     auto waves = [&](int h) { return (int)(((int64_t)tokens * h + (int64_t)per_wave * passes - 1) / ((int64_t)per_wave * passes)); };
     const int q_waves = waves(heads), k_waves = waves(heads_kv);

@@ -359,8 +359,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendPa
 
 // The vector form: a lane has eight consecutive elements of a row (16 bytes), a wave 512 / dim rows at a time, rows of one kind (query,
 // key, value) counted through all tokens so that few kv heads still fill the wave.  The other half of a rotated pair lies rotary_dim / 16
-// lanes away: its raw elements come over as four dwords, and the lane norms them itself.  The next rows are requested before the
-// present ones are worked on; tables are read again only when the token changes.
+// lanes away: its raw elements come over as four dwords, and the lane norms them itself.  All rows of a wave are requested at its
+// start; tables are read again only when the token changes.
 // Takes: rotary_dim a multiple of 16 (interleaved: of 8), rows, tables and weights 16-byte aligned.
 // Bound: memory.
 // Four values (16-bit or fp32) of a weight or table as floats.
@@ -519,13 +519,20 @@ __device__ __forceinline__ void store_cached(const AppendParams& p, void* cache,
 
 enum { kQuery, kKey, kValue };
 
+// Rows of large calls stream past the caches (8192 tokens: 71 -> 65 us); the few of a decode step stay there for the attention that follows.
+template <int PASSES> __device__ __forceinline__ u32x4 load_once(const u32x4* p) { return PASSES > 1 ? __builtin_nontemporal_load(p) : *p; }
+template <int PASSES> __device__ __forceinline__ void store_once(u32x4* p, u32x4 v) {
+  if constexpr (PASSES > 1) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
 // Rows of one kind.  R: the type that norm and rotation are formed in (see the general form).
-template <typename XT, int CACHE, int KIND, typename R>
-__device__ __forceinline__ void append_rows(const AppendParams& p, int wave, int passes) {
+template <typename XT, int CACHE, int KIND, typename R, int PASSES>
+__device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
   const int lane = threadIdx.x & 63;
   const int lanes = p.dim >> 3, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
   const int heads = KIND == kQuery ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^30: the launcher checks)
-  const int row0 = wave * passes * per_wave;
+  const int row0 = wave * PASSES * per_wave;
   if (row0 >= rows) return;
   const uint16_t* base = KIND == kQuery ? p.q : KIND == kKey ? p.k : p.v;
   const int64_t stride = KIND == kQuery ? p.q_stride : KIND == kKey ? p.k_stride : p.v_stride;
@@ -538,36 +545,62 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave, int
   turn.mate = turn.on && !p.interleaved ? (turn.upper ? j - apart : j + apart) : j;
   const int mate_lane = lane - j + turn.mate;
 
-  // the lane's row of the pass that is requested next: token and head, stepped instead of divided
+  // the lane's rows, all requested at once: token and head, stepped instead of divided
   const int dt = per_wave / heads, dh = per_wave - dt * heads;
-  int token = (row0 + lane / lanes) / heads, head = row0 + lane / lanes - token * heads;
   const R inv_dim = (R)1 / (R)p.dim;  // (a power of two)
-  auto request = [&]() __attribute__((always_inline)) -> u32x4 {
-    const int t = min(token, p.tokens - 1);  // (past the end: a row of the last token again, which is not stored)
-    return *(const u32x4*)(base + t * stride + head * p.dim + 8 * j);
-  };
-  u32x4 ahead = request();
-  int token_of_side = -1;
-  f32x4 wc[2], ws[2];  // weight times cosine, the other half's weight times sine
-  for (int i = 0; i < passes; i++) {
-    if (row0 + i * per_wave >= rows) break;
-    const int r = row0 + i * per_wave + lane / lanes, t = min(token, p.tokens - 1), h = head;
-    const uint32_t x[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
-    token += dt;
-    head += dh;
-    if (head >= heads) {
-      head -= heads;
-      token++;
+  int tokens[PASSES], head_of[PASSES];
+  u32x4 raw[PASSES];
+  {
+    int token = (row0 + lane / lanes) / heads, head = row0 + lane / lanes - token * heads;
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+      tokens[i] = min(token, p.tokens - 1);  // (past the end: a row of the last token again, which is not stored)
+      head_of[i] = head;
+      raw[i] = load_once<PASSES>((const u32x4*)(base + tokens[i] * stride + head * p.dim + 8 * j));
+      token += dt;
+      head += dh;
+      if (head >= heads) {
+        head -= heads;
+        token++;
+      }
     }
-    if (i + 1 < passes) ahead = request();
-    int64_t slot = 0;
-    if constexpr (KIND != kQuery) slot = p.slots[t];
+  }
+  // What depends on the token is requested here too, ahead of all stores (which the compiler keeps loads behind).
+  int64_t slots[PASSES], tpos[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; i++) {
+    slots[i] = KIND != kQuery ? p.slots[tokens[i]] : 0;
+    tpos[i] = rotates ? min(max(p.positions[tokens[i]], 0), p.max_position - 1) : 0;  // never outside the tables
+  }
+  // 64-bit rows: tables and weights as they are; 32-bit rows: weight times cosine, the other half's weight times sine
+  constexpr bool WIDE = sizeof(R) == 8;
+  f32x4 c[WIDE ? PASSES : 1][2], s[WIDE ? PASSES : 1][2], w[2], wo[2];
+  if constexpr (KIND != kValue) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      w[k] = wo[k] = f32x4{1.f, 1.f, 1.f, 1.f};
+      if (weight) {
+        w[k] = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32);
+        wo[k] = p.interleaved ? f32x4{w[k][1], w[k][0], w[k][3], w[k][2]} : load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
+      }
+#pragma unroll
+      for (int i = 0; i < (WIDE ? PASSES : 1); i++) side4<XT>(p, turn, tpos[i], j, k, &c[i][k], &s[i][k]);
+      if constexpr (!WIDE) {
+        c[0][k] *= w[k];
+        s[0][k] *= wo[k];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; i++) {
+    if (row0 + i * per_wave >= rows) break;
+    const int r = row0 + i * per_wave + lane / lanes, t = tokens[i], h = head_of[i];
+    const uint32_t x[4] = {raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
+    const int64_t slot = slots[i];
     float y[8];
     if constexpr (KIND == kValue) {
       Unpack<XT, 8>::run(x, y);
     } else {
-      int64_t tpos = 0;
-      if (rotates) tpos = min(max(p.positions[t], 0), p.max_position - 1);  // never outside the tables
       uint32_t other[4];
       if (rotates) {
         if (p.interleaved) {
@@ -588,67 +621,65 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave, int
         sum = over_row(sum, lanes, [](R a, R b) { return a + b; });
         rstd = inverse_root(sum * inv_dim + (R)p.eps);
       }
-      if constexpr (sizeof(R) == 4) {
-        if (i == 0 || (rotates && __ballot(t != token_of_side))) {
-          token_of_side = t;
+      float of[8];
+      if (rotates) Unpack<XT, 8>::run(other, of);
+      if constexpr (!WIDE) {
+        if (i > 0 && rotates && __ballot(t != tokens[i > 0 ? i - 1 : 0])) {  // another token's tables
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            side4<XT>(p, turn, tpos, j, k, &wc[k], &ws[k]);
-            if (weight) {
-              const f32x4 w = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32), wo = load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
-              wc[k] *= w;
-              ws[k] *= p.interleaved ? f32x4{w[1], w[0], w[3], w[2]} : wo;
-            }
+            side4<XT>(p, turn, tpos[i], j, k, &c[0][k], &s[0][k]);
+            c[0][k] *= w[k];
+            s[0][k] *= wo[k];
           }
         }
-        float of[8];
-        if (rotates) Unpack<XT, 8>::run(other, of);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          float z = xf[e] * wc[e >> 2][e & 3];
-          if (rotates) z = __builtin_fmaf(of[e], ws[e >> 2][e & 3], z);
+          float z = xf[e] * c[0][e >> 2][e & 3];
+          if (rotates) z = __builtin_fmaf(of[e], s[0][e >> 2][e & 3], z);
           y[e] = z * rstd;
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          f32x4 c, s, w = {1.f, 1.f, 1.f, 1.f}, wo = w;
-          side4<XT>(p, turn, tpos, j, k, &c, &s);
-          if (weight) {
-            w = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32);
-            wo = p.interleaved ? f32x4{w[1], w[0], w[3], w[2]} : load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
-          }
-          float of[4] = {0.f, 0.f, 0.f, 0.f};
-          if (rotates) Unpack<XT, 4>::run(other + 2 * k, of);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            R z = (R)xf[4 * k + e] * (R)w[e] * (R)c[e];
-            if (rotates) z += (R)of[e] * (R)wo[e] * (R)s[e];
-            y[4 * k + e] = (float)(z * rstd);
-          }
+        for (int e = 0; e < 8; e++) {
+          const int k = e >> 2, l = e & 3;
+          R z = (R)xf[e] * (R)w[k][l] * (R)c[WIDE ? i : 0][k][l];
+          if (rotates) z += (R)of[e] * (R)wo[k][l] * (R)s[WIDE ? i : 0][k][l];
+          y[e] = (float)(z * rstd);
         }
       }
     }
     const bool store = r < rows && (KIND == kQuery || (slot >= 0 && slot < p.n_tokens));
     if constexpr (KIND == kQuery) {
-      if (store) *(u32x4*)(p.q_out + (int64_t)r * p.dim + 8 * j) = pack_row8<XT>(y);
+      if (store) store_once<PASSES>((u32x4*)(p.q_out + (int64_t)r * p.dim + 8 * j), pack_row8<XT>(y));
     } else {
       store_cached<XT, CACHE>(p, KIND == kKey ? p.k_cache : p.v_cache, KIND == kKey ? p.k_scale : p.v_scale, y, slot, h, lanes, j, store);
     }
   }
 }
 
-template <typename XT, int CACHE>
-__global__ __launch_bounds__(256, 4) void qk_norm_rope_append_rows_kernel(const AppendParams p, int passes, int q_waves, int k_waves) {
+// PASSES of a wave over query rows; key and value rows, whose token changes more often, take half as many.
+template <typename XT, int CACHE, int PASSES>
+__global__ __launch_bounds__(256, 4) void qk_norm_rope_append_rows_kernel(const AppendParams p, int q_waves, int k_waves) {
+  constexpr int KP = (PASSES + 1) / 2;
   int wave = blockIdx.x * 4 + uni(threadIdx.x >> 6);
   if (wave < k_waves) {  // (the longest rows first)
-    if constexpr (CACHE == kCache16) append_rows<XT, CACHE, kKey, float>(p, wave, passes);
-    else append_rows<XT, CACHE, kKey, double>(p, wave, passes);
+    if constexpr (CACHE == kCache16) append_rows<XT, CACHE, kKey, float, KP>(p, wave);
+    else append_rows<XT, CACHE, kKey, double, KP>(p, wave);
   } else if ((wave -= k_waves) < q_waves) {
-    append_rows<XT, CACHE, kQuery, float>(p, wave, passes);
+    append_rows<XT, CACHE, kQuery, float, PASSES>(p, wave);
   } else {
-    append_rows<XT, CACHE, kValue, float>(p, wave - q_waves, passes);
+    append_rows<XT, CACHE, kValue, float, KP>(p, wave - q_waves);
   }
+}
+
+template <typename XT, int PASSES>
+void launch_append_rows(const AppendParams& p, int cache, hipStream_t s) {
+  auto waves = [&](int heads, int rows) { return (int)(((int64_t)p.tokens * heads + rows - 1) / rows); };
+  const int q_waves = waves(p.heads, 512 / p.dim * PASSES), k_waves = waves(p.heads_kv, 512 / p.dim * ((PASSES + 1) / 2));
+  const dim3 grid((q_waves + 2 * k_waves + 3) / 4), block(256);
+  auto kern = cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp4, PASSES>
+              : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp8, PASSES> : qk_norm_rope_append_rows_kernel<XT, kCache16, PASSES>;
+  hipLaunchKernelGGL(kern, grid, block, 0, s, p, q_waves, k_waves);
 }
 
 // --------------------------------------------------------------------------------------------- rows of the 4-bit cache
@@ -764,16 +795,9 @@ const char* launch_qk_norm_rope_append(const void* q, const void* k, const void*
   const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table | (uintptr_t)sin_table;
   const int64_t most_rows = (int64_t)tokens * (heads > heads_kv ? heads : heads_kv);
   if (rotary_dim % (interleaved ? 8 : 16) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 30)) {
-    const int per_wave = 512 / dim;
-    const int passes = append_passes(tokens, heads, heads_kv, per_wave);
-    auto waves = [&](int h) { return (int)(((int64_t)tokens * h + (int64_t)per_wave * passes - 1) / ((int64_t)per_wave * passes)); };
-    const int q_waves = waves(heads), k_waves = waves(heads_kv);
-    const dim3 grid((q_waves + 2 * k_waves + 3) / 4), block(256);
-    auto kern = bf16 ? (cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<bf16_tag, kCacheFp4>
-                        : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<bf16_tag, kCacheFp8> : qk_norm_rope_append_rows_kernel<bf16_tag, kCache16>)
-                     : (cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<fp16_tag, kCacheFp4>
-                        : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<fp16_tag, kCacheFp8> : qk_norm_rope_append_rows_kernel<fp16_tag, kCache16>);
-    hipLaunchKernelGGL(kern, grid, block, 0, s, p, passes, q_waves, k_waves);
+    const bool many = append_passes(tokens, heads, heads_kv, 512 / dim) > 1;
+    if (bf16) many ? launch_append_rows<bf16_tag, 4>(p, cache, s) : launch_append_rows<bf16_tag, 1>(p, cache, s);
+    else many ? launch_append_rows<fp16_tag, 4>(p, cache, s) : launch_append_rows<fp16_tag, 1>(p, cache, s);
     return launched();
   }
   const dim3 grid(tokens, (heads + 2 * heads_kv + 3) / 4), block(256);

@@ -861,3 +861,144 @@ def test_compiled_step_equals_the_eager_one():
     leaf = args[0].clone().requires_grad_()
     with pytest.raises(RuntimeError):
         op(leaf, *args[1:]).sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------------- the native host path
+class _Calls:
+    """``native._hostcall`` with a record of what it took."""
+
+    def __init__(self, module):
+        self.module, self.taken = module, []
+
+    def __getattr__(self, name):
+        function = getattr(self.module, name)
+
+        def call(*args):
+            out = function(*args)
+            self.taken.append((name, out is not None))
+            return out
+
+        return call
+
+
+def _host_cases():
+    """(op, arguments, indices of the arguments that it writes), on the device."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    cases = [
+        (AllocOp(3, 4, 16, 9), [_int([0, 16, 3]), _int([[0] * 4, [7] * 4, [8] * 4]), _int(list(range(9))), _int([6])], (1,)),
+        (AllocOp(3, 4, 16, 9), [_int([0, 16, 3]), _int([[0] * 9, [7] * 9, [8] * 9])[:, :4], _int(list(range(9))), _int([6]), _int([0, 20, 20, 23]), 30], (1,)),
+        (ReleaseOp(2, 4, 16, 9), [torch.tensor([True, False], device=DEV), _int([20, 3]), _int([[3, 4, 0, 0], [5, 0, 0, 0]]), _int(list(range(9))), _int([2])], (3,)),
+    ]
+    for cache, written in ((FP4, (9, 10, 11, 12)), (FP8, (9, 10, 11, 12)), (None, (9, 10))):
+        a = _append_args(cache, device=DEV)
+        for t in a.values():
+            if t is not None and t.is_floating_point() and t.dtype != FP8:
+                t.copy_(torch.randn(t.shape, generator=g, device=DEV))
+        a["slot_mapping"].copy_(torch.tensor([5, -1, 17], device=DEV))
+        order = [*list(a)[:9], "k_cache", "v_cache", "k_scale", "v_scale"]
+        cases.append((AppendOp(4, 2, 128, 16, cache_dtype=cache), [a[n] for n in order if n in a], written))
+    d = _decode_args(device=DEV)
+    for name in ("k", "v"):
+        d[name].copy_(torch.randint(0, 256, d[name].shape, generator=g, device=DEV, dtype=torch.uint8))
+    d["q"].copy_(torch.randn(d["q"].shape, generator=g, device=DEV))
+    d["real_seqlen_kv"].copy_(_int([30, 17]))
+    cases += [(GatherOp(2, 128, 16), [d["k"], d["v"], d["k_scale"], d["v_scale"], torch.tensor([3, -1, 40], device=DEV)], ()),
+              (FP4DecodeOp(2, 4, 2, 64, 128, 16), list(d.values()), ())]
+    return cases
+
+
+def _clone(x):
+    return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device).copy_(x) if isinstance(x, torch.Tensor) else x
+
+
+def _bytes(x):
+    return [t.contiguous().view(torch.uint8) for t in (x if isinstance(x, tuple) else (x,)) if isinstance(t, torch.Tensor)]
+
+
+@pytest.mark.gpu
+def test_native_host_calls_equal_the_registered_operators(monkeypatch):
+    """The first call goes through the operator registry, the second through the native path: same outputs, same memory written, and the
+    written tensors -- no others -- have a new version either way."""
+    require_gfx950()
+    native.hostcall()
+    for op, args, written in _host_cases():
+        calls = _Calls(native.hostcall())
+        monkeypatch.setattr(native, "_hostcall", calls)
+        seen = []
+        for _ in range(2):
+            mine = [_clone(x) for x in args]
+            versions = [x._version if isinstance(x, torch.Tensor) else 0 for x in mine]
+            out = op(*mine)
+            raised = [i for i, x in enumerate(mine) if isinstance(x, torch.Tensor) and x._version > versions[i]]
+            seen.append((_bytes(out), _bytes(tuple(mine)), raised))
+        monkeypatch.setattr(native, "_hostcall", calls.module)
+        assert [ok for _, ok in calls.taken] == [True], (type(op).__name__, calls.taken)
+        assert all(torch.equal(a, b) for i in (0, 1) for a, b in zip(seen[0][i], seen[1][i], strict=True)), type(op).__name__
+        assert seen[0][2] == seen[1][2] == list(written), (type(op).__name__, seen[0][2], seen[1][2])
+
+
+@pytest.mark.gpu
+def test_calls_that_the_native_host_path_leaves_to_python(monkeypatch):
+    """After a good call: every refusal still speaks, subclasses and dispatch modes still see the operator, other kernels still serve."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    require_gfx950()
+    native.hostcall()
+
+    class Names(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Sub(torch.Tensor):
+        pass
+
+    for op, args, _ in _host_cases():
+        op(*args)
+        name = type(op).__name__
+        calls = _Calls(native.hostcall())
+        monkeypatch.setattr(native, "_hostcall", calls)
+        for i, x in enumerate(args):
+            if not isinstance(x, torch.Tensor):
+                continue
+            wrong = [x.cpu(), x.to(torch.float64), x.unsqueeze(0), [1]]
+            if not (isinstance(op, GatherOp) and i == 4):  # no rows are a good call
+                wrong.append(x[:0])
+            for bad in wrong:
+                with pytest.raises(ValueError):
+                    op(*args[:i], bad, *args[i + 1:])
+        assert not any(ok for _, ok in calls.taken), name
+        with Names() as mode:
+            op(*args)
+        assert any(n.startswith(op.compile_op_names[0].replace("::", ".")) for n in mode.names), (name, mode.names)
+        op(*(x.as_subclass(Sub) if isinstance(x, torch.Tensor) else x for x in args))
+        assert not any(ok for _, ok in calls.taken), name
+        leaf = [x.clone().requires_grad_() if isinstance(x, torch.Tensor) and x.dtype in (BF16, torch.float32) else x for x in args]
+        if any(isinstance(x, torch.Tensor) and x.requires_grad for x in leaf):
+            with torch.no_grad():
+                op(*leaf)
+            assert calls.taken[-1][1], name
+        op(*args)
+        assert calls.taken[-1][1], name
+        monkeypatch.setattr(native, "_hostcall", calls.module)
+
+
+@pytest.mark.gpu
+def test_another_kernel_class_is_not_passed_by():
+    """A kernel map given, or changed after calls, decides who serves."""
+    require_gfx950()
+    op, args, _ = _host_cases()[-1]
+    want = op(*args)
+    assert torch.equal(op(*args), want)
+    key = op._key
+
+    class Mine(op.kernel_map[key]):
+        def forward(self, *a):
+            return super().forward(*a) + 1
+
+    op.kernel_map[key] = Mine
+    assert torch.equal(op(*args), want + 1)

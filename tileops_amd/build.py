@@ -1,7 +1,8 @@
 """Build libmi355_tileops.so (HIP kernels + C ABI) for gfx950 with hipcc, in-tree.
 
 ``python -m tileops_amd.build`` compiles every translation unit under ``tileops_amd/csrc`` and links
-``tileops_amd/lib/libmi355_tileops.so``.  hipcc cross-compiles, so no GPU is needed to build.
+``tileops_amd/lib/libmi355_tileops.so``.  hipcc cross-compiles, so no GPU is needed to build.  Beside it goes
+``tileops_amd/lib/_hostcall.so``, the host side of the serving-step calls (a Python module on torch's C++ interface, no device code).
 """
 
 from __future__ import annotations
@@ -17,6 +18,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libmi355_tileops.so"
+HOSTCALL_PATH = LIB_DIR / "_hostcall.so"
 OBJ_DIR = PKG / "build"
 
 SOURCES = ["abi.hip", "paged_decode_generic.hip", "paged_decode_mfma.hip", "paged_cache_utils.hip", "paged_cache_step.hip",
@@ -73,5 +75,35 @@ def build(verbose: bool = True, extra_flags: tuple = (), lib_path: Path = LIB_PA
     return lib_path
 
 
+def build_hostcall(verbose: bool = True) -> Path:
+    """Compile ``csrc/hostcall.cpp`` against torch and the library (built before)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler found; the host side of the serving-step calls cannot be built")
+    tmp = HOSTCALL_PATH.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in (*cpp_extension.include_paths(), sysconfig.get_path("include")):
+        cmd += ["-isystem", path]
+    cmd += [str(CSRC / "hostcall.cpp"), "-o", str(tmp), "-L", str(LIB_DIR), "-lmi355_tileops"]
+    for path in cpp_extension.library_paths():
+        cmd += ["-L", path]
+    cmd += ["-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling hostcall.cpp failed:\n{res.stderr}")
+    if res.stderr.strip():
+        print(res.stderr, file=sys.stderr)
+    os.replace(tmp, HOSTCALL_PATH)
+    if verbose:
+        print(f"built {HOSTCALL_PATH} ({HOSTCALL_PATH.stat().st_size} bytes)")
+    return HOSTCALL_PATH
+
+
 if __name__ == "__main__":
     build()
+    build_hostcall()

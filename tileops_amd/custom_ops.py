@@ -16,10 +16,6 @@ kernel class's ``forward`` goes through one of the operators below.  Each operat
 Operator names: ``tileops_amd::gqa_paged_decode``, ``tileops_amd::gqa_decode``, ``tileops_amd::gqa_prefill_paged``,
 ``tileops_amd::gqa_prefill_paged_rope``, and of a serving step around a paged cache ``tileops_amd::kv_alloc``, ``tileops_amd::kv_release``,
 ``tileops_amd::qk_norm_rope_append``, ``tileops_amd::kv_gather_fp4``, ``tileops_amd::gqa_paged_decode_fp4``.
-
-An operator call through torch's dispatcher costs the host about 30 us, several times what the kernels of a decode step's
-bookkeeping run.  The serving-step kernel classes therefore call the implementations below (``*_impl``) directly where the dispatcher
-has nothing to add -- plain tensors outside any tracing, see ``plain_call``.
 """
 
 from __future__ import annotations
@@ -31,7 +27,7 @@ import torch
 from . import native
 
 __all__ = ["OP_NAMES", "gqa_decode", "gqa_paged_decode", "gqa_paged_decode_fp4", "gqa_prefill_paged", "gqa_prefill_paged_rope", "kv_alloc",
-           "kv_gather_fp4", "kv_release", "plain_call", "qk_norm_rope_append"]
+           "kv_gather_fp4", "kv_release", "qk_norm_rope_append"]
 
 OP_NAMES = ("tileops_amd::gqa_paged_decode", "tileops_amd::gqa_decode", "tileops_amd::gqa_prefill_paged",
             "tileops_amd::gqa_prefill_paged_rope", "tileops_amd::kv_alloc", "tileops_amd::kv_release", "tileops_amd::qk_norm_rope_append",
@@ -154,20 +150,10 @@ def _(q, k_new, v_new, k_pages, v_pages, cos_table, sin_table, cu_seqlens_q, cac
 
 
 # --- a serving step around a paged cache ------------------------------------------------------------------------------------
-def plain_call(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether a call on *tensors* needs nothing of torch's dispatcher: no tracing, no dispatch mode, no tensor subclass, no gradient."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
-        return False
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or (grad and t.requires_grad)):
-            return False
-    return True
-
-
-def kv_alloc_impl(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-                  cu_seqlens_q: Optional[torch.Tensor], total_q: int, page_size: int
-                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+@torch.library.custom_op("tileops_amd::kv_alloc", mutates_args=("block_table",))
+def kv_alloc(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+             cu_seqlens_q: Optional[torch.Tensor], total_q: int, page_size: int
+             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Pages and slots of a step's new tokens (``mi355_kv_alloc``); writes the new entries of ``block_table``."""
     native.require_gfx950(block_table.device)
     outs = _kv_alloc_outputs(cache_seqlens, total_q)
@@ -182,16 +168,14 @@ def _kv_alloc_outputs(cache_seqlens, total_q):
             torch.empty(1, dtype=torch.int32, device=device))
 
 
-kv_alloc = torch.library.custom_op("tileops_amd::kv_alloc", kv_alloc_impl, mutates_args=("block_table",))
-
-
 @kv_alloc.register_fake
 def _(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q, page_size):
     return _kv_alloc_outputs(cache_seqlens, total_q)
 
 
-def kv_release_impl(finished: torch.Tensor, seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-                    page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+@torch.library.custom_op("tileops_amd::kv_release", mutates_args=("free_pages",))
+def kv_release(finished: torch.Tensor, seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+               page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Pages of finished sequences back onto the list (``mi355_kv_release``); writes ``free_pages`` behind its free ones."""
     native.require_gfx950(block_table.device)
     outs = (torch.empty_like(seqlens), torch.empty_like(free_count))
@@ -199,19 +183,17 @@ def kv_release_impl(finished: torch.Tensor, seqlens: torch.Tensor, block_table: 
     return outs
 
 
-kv_release = torch.library.custom_op("tileops_amd::kv_release", kv_release_impl, mutates_args=("free_pages",))
-
-
 @kv_release.register_fake
 def _(finished, seqlens, block_table, free_pages, free_count, page_size):
     return torch.empty_like(seqlens), torch.empty_like(free_count)
 
 
-def qk_norm_rope_append_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
-                             cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], positions: Optional[torch.Tensor],
-                             slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor],
-                             v_scale: Optional[torch.Tensor], rotary_dim: int, interleaved: bool, eps: float, page_size: int,
-                             cache_code: int) -> torch.Tensor:
+@torch.library.custom_op("tileops_amd::qk_norm_rope_append", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                        cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                        slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor],
+                        v_scale: Optional[torch.Tensor], rotary_dim: int, interleaved: bool, eps: float, page_size: int,
+                        cache_code: int) -> torch.Tensor:
     """Norm + rotation of query and key rows, append of keys and values (``mi355_qk_norm_rope_append``)."""
     native.require_gfx950(q.device)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -220,18 +202,15 @@ def qk_norm_rope_append_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return out
 
 
-qk_norm_rope_append = torch.library.custom_op("tileops_amd::qk_norm_rope_append", qk_norm_rope_append_impl,
-                                              mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
-
-
 @qk_norm_rope_append.register_fake
 def _(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, rotary_dim, interleaved,
       eps, page_size, cache_code):
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
-def kv_gather_fp4_impl(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
-                       dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+@torch.library.custom_op("tileops_amd::kv_gather_fp4", mutates_args=())
+def kv_gather_fp4(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
+                  dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of a 4-bit cache as 16-bit values (``mi355_kv_gather_fp4``)."""
     native.require_gfx950(k.device)
     outs = _kv_gather_outputs(k, slot_mapping, dtype)
@@ -244,9 +223,6 @@ def _kv_gather_outputs(k, slot_mapping, dtype):
     return torch.empty(shape, dtype=dtype, device=k.device), torch.empty(shape, dtype=dtype, device=k.device)
 
 
-kv_gather_fp4 = torch.library.custom_op("tileops_amd::kv_gather_fp4", kv_gather_fp4_impl, mutates_args=())
-
-
 @kv_gather_fp4.register_fake
 def _(k, v, k_scale, v_scale, slot_mapping, dtype):
     return _kv_gather_outputs(k, slot_mapping, dtype)
@@ -255,9 +231,10 @@ def _(k, v, k_scale, v_scale, slot_mapping, dtype):
 _decode_fp4_plans: dict[tuple, int] = {}
 
 
-def gqa_paged_decode_fp4_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
-                              real_seqlen_kv: torch.Tensor, block_table: torch.Tensor, q_len: int, heads: int, heads_kv: int, dim: int,
-                              page_size: int, sm_scale: float, softcap: float, causal: bool) -> torch.Tensor:
+@torch.library.custom_op("tileops_amd::gqa_paged_decode_fp4", mutates_args=())
+def gqa_paged_decode_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                         real_seqlen_kv: torch.Tensor, block_table: torch.Tensor, q_len: int, heads: int, heads_kv: int, dim: int,
+                         page_size: int, sm_scale: float, softcap: float, causal: bool) -> torch.Tensor:
     """Paged GQA decode over a 4-bit cache (``mi355_gqa_paged_decode_fp4``)."""
     native.require_gfx950(q.device)
     batch = q.shape[0]
@@ -270,9 +247,6 @@ def gqa_paged_decode_fp4_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                             q_len=q_len, heads=heads, heads_kv=heads_kv, dim=dim, page_size=page_size, sm_scale=sm_scale, softcap=softcap,
                             causal=causal)
     return out
-
-
-gqa_paged_decode_fp4 = torch.library.custom_op("tileops_amd::gqa_paged_decode_fp4", gqa_paged_decode_fp4_impl, mutates_args=())
 
 
 @gqa_paged_decode_fp4.register_fake

@@ -8,13 +8,15 @@ or the device is not a gfx950 GPU, calls raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
-from typing import Optional
+from typing import Any, Optional
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmi355_tileops.so"
+HOSTCALL_PATH = LIB_PATH.with_name("_hostcall.so")
 ABI_VERSION = 1
 
 DT_BF16, DT_FP16, DT_FP8_E4M3FN, DT_FP32, DT_FP4_E2M1 = 0, 1, 2, 3, 4
@@ -52,6 +54,7 @@ class NativeLibraryError(RuntimeError):
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
+_hostcall: Any = None
 _facts_local = threading.local()  # per-thread pinned buffer of prefill_input_facts
 
 _c_int, _c_i64, _c_f32, _c_vp, _c_sz = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
@@ -163,6 +166,24 @@ def load() -> ctypes.CDLL:
             raise NativeLibraryError(f"{LIB_PATH} has ABI version {got}, this package expects {ABI_VERSION}; rebuild")
         _lib = lib
         return lib
+
+
+def hostcall() -> Any:
+    """The module that checks, allocates for and enqueues a serving-step call on plain tensors in one native call
+    (csrc/hostcall.cpp).  Loaded once, after the library that it calls."""
+    global _hostcall
+    if _hostcall is not None:
+        return _hostcall
+    load()
+    with _lock:
+        if _hostcall is None:
+            if not HOSTCALL_PATH.exists():
+                raise NativeLibraryError(f"{HOSTCALL_PATH} is missing: build it with `python -m tileops_amd.build`")
+            spec = importlib.util.spec_from_file_location("_hostcall", HOSTCALL_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _hostcall = module
+    return _hostcall
 
 
 def last_error() -> str:

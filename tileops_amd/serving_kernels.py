@@ -1,7 +1,8 @@
 """L1 host wrappers of the serving-step kernels: pages, append, 4-bit rows, attention over a 4-bit cache.
 
-Each class states the calls that it serves (``applies`` / ``refusal``, like every kernel class of the package) and enqueues one
-library call on the current stream.  Nothing is read back.  The reference has no counterpart of these.
+Each class states the calls that it serves (``applies`` / ``refusal``, like every kernel class of the package); ``forward`` is one
+registered operator, which enqueues one library call on the current stream.  Nothing is read back.  The reference has no counterpart
+of these.
 """
 
 from __future__ import annotations
@@ -11,7 +12,8 @@ from typing import Any, Optional
 
 import torch
 
-from . import custom_ops, native
+from . import custom_ops as _custom_ops  # noqa: F401 - registers torch.ops.tileops_amd.*
+from . import native
 from .kernels import GFX950_ARCH, Kernel
 
 __all__ = [
@@ -52,18 +54,14 @@ class PagedKVCacheAllocKernel(_ServingKernel):
     """Pages, slots and positions of a step's new tokens."""
 
     def forward(self, cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q):
-        plain = custom_ops.plain_call(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q)
-        call = custom_ops.kv_alloc_impl if plain else torch.ops.tileops_amd.kv_alloc
-        return call(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q, self.op.page_size)
+        return torch.ops.tileops_amd.kv_alloc(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q, self.op.page_size)
 
 
 class PagedKVCacheReleaseKernel(_ServingKernel):
     """Pages of finished sequences back onto the list."""
 
     def forward(self, finished, seqlens, block_table, free_pages, free_count):
-        plain = custom_ops.plain_call(finished, seqlens, block_table, free_pages, free_count)
-        call = custom_ops.kv_release_impl if plain else torch.ops.tileops_amd.kv_release
-        return call(finished, seqlens, block_table, free_pages, free_count, self.op.page_size)
+        return torch.ops.tileops_amd.kv_release(finished, seqlens, block_table, free_pages, free_count, self.op.page_size)
 
 
 class QKNormRopePagedKVAppendKernel(_ServingKernel):
@@ -74,19 +72,16 @@ class QKNormRopePagedKVAppendKernel(_ServingKernel):
         code = {FP4: native.DT_FP4_E2M1, FP8: native.DT_FP8_E4M3FN}.get(op.cache_dtype)
         if code is None:
             code = native.dtype_code(q.dtype)
-        plain = custom_ops.plain_call(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale)
-        call = custom_ops.qk_norm_rope_append_impl if plain else torch.ops.tileops_amd.qk_norm_rope_append
-        return call(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, op.rotary_dim,
-                    op.interleaved, op.eps, op.page_size, code)
+        return torch.ops.tileops_amd.qk_norm_rope_append(
+            q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale,
+            op.rotary_dim, op.interleaved, op.eps, op.page_size, code)
 
 
 class PagedFP4KVCacheGatherKernel(_ServingKernel):
     """Rows of a 4-bit cache as 16-bit values."""
 
     def forward(self, k, v, k_scale, v_scale, slot_mapping):
-        plain = custom_ops.plain_call(k, v, k_scale, v_scale, slot_mapping)
-        call = custom_ops.kv_gather_fp4_impl if plain else torch.ops.tileops_amd.kv_gather_fp4
-        return call(k, v, k_scale, v_scale, slot_mapping, self.op.dtype)
+        return torch.ops.tileops_amd.kv_gather_fp4(k, v, k_scale, v_scale, slot_mapping, self.op.dtype)
 
 
 class GQADecodePagedFP4Kernel(_ServingKernel):
@@ -98,7 +93,6 @@ class GQADecodePagedFP4Kernel(_ServingKernel):
 
     def forward(self, q, k, v, k_scale, v_scale, real_seqlen_kv, block_table):
         op = self.op
-        plain = custom_ops.plain_call(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table)
-        call = custom_ops.gqa_paged_decode_fp4_impl if plain else torch.ops.tileops_amd.gqa_paged_decode_fp4
-        return call(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table, op.q_len, op.heads, op.heads_kv, op.dim, op.page_size,
-                    float(op.sm_scale), float(op.softcap), op.is_causal)
+        return torch.ops.tileops_amd.gqa_paged_decode_fp4(
+            q, k, v, k_scale, v_scale, real_seqlen_kv, block_table, op.q_len, op.heads, op.heads_kv, op.dim, op.page_size,
+            float(op.sm_scale), float(op.softcap), op.is_causal)

@@ -19,6 +19,7 @@ from typing import Dict, Optional
 
 import torch
 
+from . import native
 from .backend import Target
 from .kernels import get_arch
 from .op_base import _UNRESOLVED, Op
@@ -65,7 +66,12 @@ def _check_table(t: torch.Tensor, device: torch.device, batch: int, width: Optio
 
 
 class _ServingOp(Op):
-    """Kernel selection that the ops of this module share: one kernel class per op."""
+    """What the ops of this module share: one kernel class per op, and the native host path.
+
+    A call goes the long way -- the checks below, kernel selection, the registered operator -- the first time, on any other device than
+    that one, under a tracer or a dispatch mode, with gradients or an external target, and whenever something is wrong with it.  Otherwise
+    ``hostcall`` (csrc/hostcall.cpp) does the same checks and the launch in one native call, or answers None: then the long way is taken.
+    """
 
     _key: str = ""
     _kernel_class: type = PagedKVCacheAllocKernel
@@ -78,7 +84,18 @@ class _ServingOp(Op):
         if target is not None:
             self.target = target
         self._selected: dict = {}
+        self._device: Optional[int] = None  # a device on which the shipped kernel has served this instance
         self.dispatch_kernel(kernel_map)
+
+    def _native(self) -> bool:
+        return (self._device is not None and self._builder is None and self.kernel_map[self._key] is self._kernel_class
+                and not torch.compiler.is_compiling())
+
+    @staticmethod
+    def _checked(result):
+        if result.__class__ is int:
+            native._check(result)
+        return result
 
     def _kernel(self, inputs: tuple, dtype: Optional[torch.dtype] = None):
         if self._builder is not None and self._builder is not _UNRESOLVED:
@@ -93,6 +110,9 @@ class _ServingOp(Op):
             kernel = self.get_or_build_kernel(key, inputs, key=(device, dtype, self.kernel_map[key]),
                                               build=lambda: self.kernel_map[key](self, device_index=index))
             self._selected[memo] = kernel
+        if self._device is None and device.type == "cuda" and device.index is not None and not torch.compiler.is_compiling():
+            native.hostcall()
+            self._device = device.index
         return kernel
 
 
@@ -127,6 +147,12 @@ class PagedKVCacheAllocFwdOp(_ServingOp):
 
     def forward(self, cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
                 cu_seqlens_q: Optional[torch.Tensor] = None, total_q: Optional[int] = None):
+        if self._native():
+            outs = native._hostcall.kv_alloc(cache_seqlens, block_table, free_pages, free_count, cu_seqlens_q, total_q, self.batch,
+                                             self.max_pages_per_req, self.num_pages, self.page_size, self._device,
+                                             torch._C._cuda_getCurrentRawStream(self._device))
+            if outs is not None:
+                return self._checked(outs)
         if not isinstance(block_table, torch.Tensor):
             raise ValueError(f"block_table must be a torch.Tensor, got {type(block_table).__name__}")
         device = block_table.device
@@ -171,6 +197,11 @@ class PagedKVCacheReleaseFwdOp(_ServingOp):
         return {"seqlens_out": (self.batch,), "free_count_out": (1,)}
 
     def forward(self, finished: torch.Tensor, seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor):
+        if self._native():
+            outs = native._hostcall.kv_release(finished, seqlens, block_table, free_pages, free_count, self.batch, self.max_pages_per_req,
+                                               self.num_pages, self.page_size, self._device, torch._C._cuda_getCurrentRawStream(self._device))
+            if outs is not None:
+                return self._checked(outs)
         if not isinstance(block_table, torch.Tensor):
             raise ValueError(f"block_table must be a torch.Tensor, got {type(block_table).__name__}")
         device = block_table.device
@@ -240,6 +271,13 @@ class QKNormRopePagedKVAppendFwdOp(_ServingOp):
                 cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], positions: Optional[torch.Tensor],
                 slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                 v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self._native():
+            out = native._hostcall.qk_norm_rope_append(
+                q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, self.heads,
+                self.heads_kv, self.dim, self.page_size, self.rotary_dim, self.interleaved, self._cache_code(q), self.eps, self._device,
+                torch._C._cuda_getCurrentRawStream(self._device))
+            if out is not None:
+                return self._checked(out)
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError(f"q must be a tensor of shape [tokens, {self.heads}, {self.dim}]")
         device, dtype, tokens = q.device, q.dtype, q.shape[0]
@@ -252,6 +290,8 @@ class QKNormRopePagedKVAppendFwdOp(_ServingOp):
         for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
             if t is None:
                 continue
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name} must be a torch.Tensor or None, got {type(t).__name__}")
             if t.dtype not in (dtype, torch.float32) or (weight_dtype or t.dtype) != t.dtype:
                 raise ValueError(f"q_weight and k_weight must both be {dtype} or both torch.float32, got {t.dtype} for {name}")
             weight_dtype = t.dtype
@@ -259,6 +299,8 @@ class QKNormRopePagedKVAppendFwdOp(_ServingOp):
         if self.rotary_dim:
             if cos_table is None or sin_table is None or positions is None:
                 raise ValueError("cos_table, sin_table and positions are required with rotary_dim > 0")
+            if not isinstance(cos_table, torch.Tensor):
+                raise ValueError(f"cos_table must be a torch.Tensor, got {type(cos_table).__name__}")
             if cos_table.dtype not in (dtype, torch.float32):
                 raise ValueError(f"cos_table must be {dtype} or torch.float32, got {cos_table.dtype}")
             if cos_table.dim() != 2 or cos_table.shape[0] < 1:
@@ -273,6 +315,16 @@ class QKNormRopePagedKVAppendFwdOp(_ServingOp):
             positions = None
         kernel = self._kernel((q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale), dtype)
         return kernel(q, k, v, q_weight, k_weight, cos_table, sin_table, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale)
+
+    def _cache_code(self, q) -> int:
+        """Type code of the cache for the native path: 0 for a cache of ``q``'s type, -1 (taken by no call) for one of another 16-bit type."""
+        if self.cache_dtype is None:
+            return 0
+        if self.cache_dtype == FP4:
+            return native.DT_FP4_E2M1
+        if self.cache_dtype == FP8:
+            return native.DT_FP8_E4M3FN
+        return 0 if getattr(q, "dtype", None) == self.cache_dtype else -1
 
     def _check_caches(self, device, dtype, k_cache, v_cache, k_scale, v_scale) -> None:
         if not isinstance(k_cache, torch.Tensor) or k_cache.dim() < 1 or k_cache.shape[0] < 1:
@@ -327,6 +379,12 @@ class PagedFP4KVCacheGatherFwdOp(_ServingOp):
         return {"k_out": shape, "v_out": shape}
 
     def forward(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor):
+        if self._native():
+            outs = native._hostcall.kv_gather_fp4(k, v, k_scale, v_scale, slot_mapping, self.heads_kv, self.dim, self.page_size,
+                                                  native.DT_BF16 if self.dtype == torch.bfloat16 else native.DT_FP16, self._device,
+                                                  torch._C._cuda_getCurrentRawStream(self._device))
+            if outs is not None:
+                return self._checked(outs)
         if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.shape[0] < 1:
             raise ValueError(f"k must have shape [n_pages, {self.heads_kv}, {self.page_size}, {self.dim // 2}]")
         _check_fp4_cache(k.device, k.shape[0], self.heads_kv, self.page_size, self.dim, k, v, k_scale, v_scale)
@@ -362,7 +420,8 @@ class GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp(_ServingOp):
             raise ValueError("seqlen_kv must be divisible by page_size")
         self.batch, self.heads, self.heads_kv, self.seqlen_kv, self.dim = batch, heads, heads_kv, seqlen_kv, dim
         self.page_size, self.q_len, self.is_causal = page_size, q_len, bool(is_causal)
-        self.sm_scale, self.softcap = _attention_scale(dim, sm_scale), _score_softcap(softcap)
+        self.sm_scale, self.softcap = float(_attention_scale(dim, sm_scale)), float(_score_softcap(softcap))
+        self._plans: dict = {}
         self._install(kernel_map, target)
 
     def _infer_output_shapes(self, q_shape, k_shape, v_shape, k_scale_shape, v_scale_shape, real_seqlen_kv_shape,
@@ -376,6 +435,17 @@ class GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp(_ServingOp):
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                 real_seqlen_kv: torch.Tensor, block_table: torch.Tensor) -> torch.Tensor:
+        if self._native():
+            dtype = getattr(q, "dtype", None)
+            plan = self._plans.get(dtype)  # workspace bytes and type code
+            if plan is not None:
+                out = native._hostcall.decode_fp4(
+                    k, v, k_scale, v_scale, q, real_seqlen_kv, block_table, self.batch, self.q_len, self.heads, self.heads_kv,
+                    self.seqlen_kv // self.page_size, self.dim, self.page_size, self.is_causal, self.sm_scale, self.softcap, *plan, self._device,
+                    torch._C._cuda_getCurrentRawStream(self._device))
+                if out is not None:
+                    self.dtype = dtype
+                    return self._checked(out)
         if not isinstance(q, torch.Tensor):
             raise ValueError(f"q must be a torch.Tensor, got {type(q).__name__}")
         device, dtype = q.device, q.dtype
@@ -385,4 +455,8 @@ class GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp(_ServingOp):
         _check("real_seqlen_kv", real_seqlen_kv, device, torch.int32, (self.batch,))
         _check_table(block_table, device, self.batch)
         self.dtype = dtype
-        return self._kernel((q, k, v, k_scale, v_scale, real_seqlen_kv, block_table), dtype)(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table)
+        kernel = self._kernel((q, k, v, k_scale, v_scale, real_seqlen_kv, block_table), dtype)
+        if self._device is not None and dtype not in self._plans:
+            self._plans[dtype] = (native.decode_fp4_workspace(self.batch, self.q_len, self.heads, self.heads_kv, self.dim, self.page_size, dtype),
+                                  native.dtype_code(dtype))
+        return kernel(q, k, v, k_scale, v_scale, real_seqlen_kv, block_table)

@@ -109,7 +109,10 @@ typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
 __device__ __forceinline__ int scalar_load(const int32_t* p, int i) { return ((scalar_ptr)(uintptr_t)p)[i]; }
 
 // Stream reads: a tile is read once per row group, and never again.
-template <typename T> __device__ __forceinline__ T stream_load(const uint8_t* p) { return __builtin_nontemporal_load((const T*)p); }
+typedef const __attribute__((address_space(1))) uint8_t* global_ptr;
+template <typename T> __device__ __forceinline__ T stream_load(global_ptr p) {
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*)p);
+}
 
 // PT: a page holds whole tiles (its size is a multiple of kTile), else it holds whole blocks of sixteen tokens.
 template <typename QT, int D, int NRB, bool PT>
@@ -137,7 +140,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   // Units of all sequences, this range of them, and its first sequence.  lens holds the lengths of sequences lens_base + lane:
   // going on to the next sequence is a register read.
   int T = 0, n0 = 0, incl0 = 0, lens = 0, lens_base = 0;
-  auto read_lens = [&](int base) __attribute__((always_inline)) -> int { return base + lane < p.batch ? len_of(p, base + lane) : 0; };
+  // (no branch over lanes: where one meets the uniform ones around it, the state behind them would be kept per lane)
+  auto read_lens = [&](int base) __attribute__((always_inline)) -> int {
+    const int len = len_of(p, min(base + lane, p.batch - 1));
+    return base + lane < p.batch ? len : 0;
+  };
   for (int base = 0; base < p.batch; base += 64) {
     const int len = read_lens(base), n = units_of_len(len), incl = wave_incl_scan(n);
     if (base == 0) {
@@ -216,33 +223,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   Segment cur = segment_at(uni(b_first), uni(pre_first), u_begin);
 
   // ---- requests: the wave's tiles of all segments as one stream, one tile ahead of the products, table entries one further ----
+  // (Behind the last tile the stream goes on in the last sequence's last page: every place stays inside the pool, nothing of it is used,
+  // and the number of loads in flight is the same in every step.)
   constexpr int NPG = PT ? 1 : NB;  // table entries of a tile
   const int step_lp = kUnit / p.page_size, step_off = kUnit - step_lp * p.page_size;
-  Segment rq = cur;                // segment of the tile that is requested next,
-  int rq_tok, rq_lp, rq_off;       // its first token, and that one's logical page and offset
-  bool live = true;                // there is such a tile
-  const int32_t* rq_row = p.block_table;  // its sequence's table row
-  int id[NPG], id_off[NPG];        // its table entries and the offsets of its blocks
-  auto rq_enter = [&]() __attribute__((always_inline)) {
-    rq_tok = rq.tok;
+  int rq_b, rq_next_unit, rq_last_page;  // sequence of the tile that is requested next, first unit behind it, its last page,
+  int rq_tok, rq_end, rq_lp, rq_off;     // the tile's first token, the end of the range's, and the token's logical page and offset
+  const int32_t* rq_row;                 // the sequence's table row
+  auto rq_enter = [&](const Segment& s) __attribute__((always_inline)) {
+    rq_b = s.b;
+    rq_next_unit = s.pre + s.nu;
+    rq_last_page = s.last_page;
+    rq_tok = s.tok;
+    rq_end = s.tok_end;
     rq_lp = rq_tok / p.page_size;
     rq_off = rq_tok - rq_lp * p.page_size;
-    rq_row = p.block_table + (int64_t)rq.b * p.bt_row_stride;
+    rq_row = p.block_table + (int64_t)s.b * p.bt_row_stride;
   };
   auto rq_settle = [&]() __attribute__((always_inline)) {  // on to a segment that has a tile for this wave
-    while (rq_tok >= rq.tok_end) {
-      const int u_next = rq.pre + rq.nu;
-      if (u_next >= u_end) {
-        live = false;
+    while (rq_tok >= rq_end) {
+      if (rq_next_unit >= u_end) {
+        rq_end = INT_MAX;
         return;
       }
-      rq = segment_at(rq.b + 1, u_next, u_next);
-      rq_enter();
+      rq_enter(segment_at(rq_b + 1, rq_next_unit, rq_next_unit));
     }
+  };
+  int id[NPG], id_off[NPG];  // table entries of a tile and the offsets of its blocks in their pages
+  auto rq_entries = [&]() __attribute__((always_inline)) {
     int lp = rq_lp, off = rq_off;
 #pragma unroll
     for (int i = 0; i < NPG; i++) {
-      id[i] = scalar_load(rq_row, min(lp, rq.last_page));  // (past the sequence's end: its last page again)
+      id[i] = scalar_load(rq_row, min(lp, rq_last_page));  // (past the sequence's end: its last page again)
       id_off[i] = off;
       off += 16;
       if (off == p.page_size) {
@@ -252,88 +264,103 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     }
   };
   int64_t at[NPG];  // byte offset of each block of the requested tile in the codes
-  auto rq_next = [&]() __attribute__((always_inline)) {
-    if (!live) return;  // (the last tile is requested again: the count of loads in flight stays the same)
+  auto rq_place = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NPG; i++) {
       const uint32_t page = (uint32_t)min(max(id[i], 0), p.n_pages - 1);
       at[i] = (int64_t)((uint64_t)page * page_bytes) + head_bytes + id_off[i] * ROW;
     }
+  };
+  auto rq_step = [&]() __attribute__((always_inline)) {
     rq_tok += kUnit;
     rq_lp += step_lp;
     rq_off += step_off;
-    if (rq_off >= p.page_size) {
-      rq_off -= p.page_size;
-      rq_lp++;
-    }
-    rq_settle();
+    const bool turn = rq_off >= p.page_size;
+    rq_off -= turn ? p.page_size : 0;
+    rq_lp += turn ? 1 : 0;
+    if (rq_tok >= rq_end) rq_settle();
+    rq_entries();
+  };
+  // (a base kept in scalar registers: the loads add the lane's 32-bit offset themselves)
+  auto base_of = [](const uint8_t* p, int64_t o) __attribute__((always_inline)) -> global_ptr {
+    global_ptr at = (global_ptr)(uintptr_t)(p + o);
+    asm("" : "+s"(at));
+    return at;
   };
   u32x4 kr[NB][KD];
   uint32_t ksr[NB][KD], vr[NB][4][VW], vsr[NB][NS];
   auto load_k = [&]() __attribute__((always_inline)) {
+    global_ptr kp, ksp;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      const int64_t o = PT ? at[0] + i * 16 * ROW : at[PT ? 0 : i];
-      const uint8_t *kp = p.k + o, *ksp = p.k_scale + (o >> 4);
+      constexpr uint32_t kStep = 16 * ROW;
+      if (!PT || i == 0) {
+        kp = base_of(p.k, at[PT ? 0 : i]);
+        ksp = base_of(p.k_scale, at[PT ? 0 : i] >> 4);
+      }
+      const uint32_t o = PT ? i * kStep : 0;
 #pragma unroll
       for (int kd = 0; kd < KD; kd++) {
-        kr[i][kd] = stream_load<u32x4>(kp + k_lane + 64 * kd);
-        ksr[i][kd] = stream_load<uint32_t>(ksp + ks_lane + 4 * kd);  // (shifted down at its use: nothing may touch it here)
+        kr[i][kd] = stream_load<u32x4>(kp + k_lane + (o + 64 * kd));
+        ksr[i][kd] = stream_load<uint32_t>(ksp + ks_lane + ((o >> 4) + 4 * kd));  // (shifted down at its use: nothing may touch it here)
       }
     }
   };
-  auto load_v = [&](int i) __attribute__((always_inline)) {
-    const int64_t o = PT ? at[0] + i * 16 * ROW : at[PT ? 0 : i];
-    const uint8_t *vp = p.v + o, *vsp = p.v_scale + (o >> 4);
+  auto load_v = [&]() __attribute__((always_inline)) {
+    global_ptr vp, vsp;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if constexpr (D == 64) vr[i][j][0] = stream_load<uint16_t>(vp + v_lane + j * ROW);
-      else if constexpr (D == 128) vr[i][j][0] = stream_load<uint32_t>(vp + v_lane + j * ROW);
-      else {
-        const u32x2 w = stream_load<u32x2>(vp + v_lane + j * ROW);
-        vr[i][j][0] = w[0];
-        vr[i][j][1] = w[1];
+    for (int i = 0; i < NB; i++) {
+      constexpr uint32_t kStep = 16 * ROW;
+      if (!PT || i == 0) {
+        vp = base_of(p.v, at[PT ? 0 : i]);
+        vsp = base_of(p.v_scale, at[PT ? 0 : i] >> 4);
       }
-    }
-    if constexpr (NS == 2) {
-      const u32x2 w = stream_load<u32x2>(vsp + vs_lane);
-      vsr[i][0] = w[0];
-      vsr[i][1] = w[1];
-    } else {
+      const uint32_t o = PT ? i * kStep : 0;
 #pragma unroll
-      for (int h = 0; h < NS / 4; h++) {
-        const u32x4 w = stream_load<u32x4>(vsp + vs_lane + 16 * h);
+      for (int j = 0; j < 4; j++) {
+        if constexpr (D == 64) vr[i][j][0] = stream_load<uint16_t>(vp + v_lane + (o + j * ROW));
+        else if constexpr (D == 128) vr[i][j][0] = stream_load<uint32_t>(vp + v_lane + (o + j * ROW));
+        else {
+          const u32x2 w = stream_load<u32x2>(vp + v_lane + (o + j * ROW));
+          vr[i][j][0] = w[0];
+          vr[i][j][1] = w[1];
+        }
+      }
+      if constexpr (NS == 2) {
+        const u32x2 w = stream_load<u32x2>(vsp + vs_lane + (o >> 4));
+        vsr[i][0] = w[0];
+        vsr[i][1] = w[1];
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) vsr[i][4 * h + e] = w[e];
+        for (int h = 0; h < NS / 4; h++) {
+          const u32x4 w = stream_load<u32x4>(vsp + vs_lane + ((o >> 4) + 16 * h));
+#pragma unroll
+          for (int e = 0; e < 4; e++) vsr[i][4 * h + e] = w[e];
+        }
       }
     }
   };
-  rq_enter();
+  rq_enter(cur);
   rq_settle();
-  if (live) {
-    rq_next();
-    load_k();
-#pragma unroll
-    for (int i = 0; i < NB; i++) load_v(i);
-  }
+  rq_entries();
+  rq_place();
+  load_k();
+  load_v();
+  rq_step();
 
   // query rows of a sequence, as they are; the next sequence's are requested before this one's results are joined
+  // (lanes behind the last row carry it once more; like all of this without a branch over lanes)
   u32x4 q_raw[NRB][D / 64][2];
   auto load_q = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int rb = 0; rb < NRB; rb++) {
-      const int r = row0 + 16 * rb + c;
-      const bool valid = r < p.rows;
-      const int s = valid ? r / p.group : 0, gi = valid ? r - s * p.group : 0;
+      const int r = min(row0 + 16 * rb + c, p.rows - 1), s = r / p.group, gi = r - s * p.group;
       const uint16_t* qp = p.q + (((int64_t)b * p.q_len + s) * p.heads + kvh * p.group + gi) * D;
       // depth positions of the lane's sixteen-byte halves h: [64h + 16g, 64h + 16g + 16) of each 128-deep step
 #pragma unroll
       for (int h = 0; h < D / 64; h++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          q_raw[rb][h][e] = u32x4{0, 0, 0, 0};
-          if (valid) q_raw[rb][h][e] = *(const u32x4*)(qp + 64 * h + 16 * g + 8 * e);
-        }
+        for (int e = 0; e < 2; e++) q_raw[rb][h][e] = *(const u32x4*)(qp + 64 * h + 16 * g + 8 * e);
     }
   };
   load_q(cur.b);
@@ -444,43 +471,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     // requested there, so a tile's reads have the rest of the step and the head of the next one to arrive.
     auto step = [&](auto masked_tag) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked_tag)::value;
+      // (products into the same accumulator are kept NRB * NB products apart: back to back each would wait for the one before)
       f32x4 s[NRB][NB];
 #pragma unroll
-      for (int rb = 0; rb < NRB; rb++)
+      for (int kd = 0; kd < KD; kd++)
 #pragma unroll
-        for (int i = 0; i < NB; i++) {
-          s[rb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NQM; n++) {
 #pragma unroll
-          for (int kd = 0; kd < KD; kd++) {
-            const u32x4 kk = kr[i][kd];
-            const i32x8 a = {(int)kk[0], (int)kk[1], (int)kk[2], (int)kk[3], 0, 0, 0, 0};
+          for (int i = 0; i < NB; i++)
 #pragma unroll
-            for (int n = 0; n < NQM; n++) {
-              const u32x4 b0 = qf[rb][kd][n][0], b1 = qf[rb][kd][n][1];
+            for (int rb = 0; rb < NRB; rb++) {
+              const u32x4 kk = kr[i][kd], b0 = qf[rb][kd][n][0], b1 = qf[rb][kd][n][1];
+              const i32x8 a = {(int)kk[0], (int)kk[1], (int)kk[2], (int)kk[3], 0, 0, 0, 0};
               const i32x8 bq = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
-              s[rb][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bq, s[rb][i], 4, 0, 0, (int)(ksr[i][kd] >> k_shift), 0, 127);
+              const f32x4 sum = kd + n == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rb][i];
+              s[rb][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bq, sum, 4, 0, 0, (int)(ksr[i][kd] >> k_shift), 0, 127);
             }
-          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-      __builtin_amdgcn_sched_barrier(0);
-      rq_next();
+      rq_place();
       load_k();
       __builtin_amdgcn_sched_barrier(0);
       uint32_t pw[NRB][NB / 2][NP][4], seen_bits[NRB][NB / 2];
       float slope[NRB], offset[NRB], top[NRB];  // logit = slope * s + offset, slope >= 0 (the sign of the softmax scale is in the query)
       bool grown = false;
+      if (softcap) {
+        // cap * tanh(x) = cap - 2 cap / (exp(2x) + 1): s becomes -1 / (exp(2x) + 1)
+#pragma unroll
+        for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+          for (int e = 0; e < 4 * NB; e++) s[rb][e >> 2][e & 3] = fast_exp2(s[rb][e >> 2][e & 3] * q_scale[rb]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+          for (int e = 0; e < 4 * NB; e++) s[rb][e >> 2][e & 3] = __builtin_amdgcn_rcpf(-1.0f - s[rb][e >> 2][e & 3]);
+      }
 #pragma unroll
       for (int rb = 0; rb < NRB; rb++) {
-        slope[rb] = q_scale[rb];
-        offset[rb] = 0.f;
-        if (softcap) {
-          // cap * tanh(x) = cap - 2 cap / (exp(2x) + 1): s becomes -1 / (exp(2x) + 1)
-#pragma unroll
-          for (int e = 0; e < 4 * NB; e++)
-            s[rb][e >> 2][e & 3] = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(s[rb][e >> 2][e & 3] * q_scale[rb]));
-          slope[rb] = 2.f * p.cap_log2e;
-          offset[rb] = p.cap_log2e;
-        }
+        slope[rb] = softcap ? 2.f * p.cap_log2e : q_scale[rb];
+        offset[rb] = softcap ? p.cap_log2e : 0.f;
         if constexpr (MASKED) {
 #pragma unroll
           for (int h = 0; h < NB / 2; h++) seen_bits[rb][h] = 0;
@@ -581,11 +611,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
             }
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        load_v(2 * h);
-        load_v(2 * h + 1);
-        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      load_v();
+      __builtin_amdgcn_sched_barrier(0);
+      rq_step();
     };
     for (; tok + kTile <= limit_min && tok < tok_end; tok += kUnit) step(std::false_type{});
     for (; tok < tok_end; tok += kUnit) step(std::true_type{});

@@ -626,6 +626,31 @@ def test_fp4_decode_over_many_sequences_and_ranges():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, q_len, dim, heads, heads_kv, page, lens, causal", [
+    (BF16, 1, 128, 8, 2, 16, [300, 0, 1, 129], True), (FP16, 1, 64, 4, 4, 48, [97, 128, 0], True), (BF16, 1, 256, 6, 2, 32, [33, 1030], True),
+    (BF16, 8, 128, 16, 2, 64, [200, 8, 31, 0, 5], True), (FP16, 17, 64, 3, 1, 16, [64, 17, 400, 3], True), (BF16, 3, 128, 7, 1, 32, [0, 2, 500], False),
+], ids=str)
+def test_fp4_decode_with_tables_of_few_and_of_many_tokens(dtype, q_len, dim, heads, heads_kv, page, lens, causal):
+    """The width of the tables, not the lengths, decides how the work is cut: both ways give the plain form's rows, at each border too."""
+    require_gfx950()
+    units = {0, 8 * 128, 16 * 128, 40000}
+    for tokens in sorted(units | {u + page for u in units}):
+        width = max(-(-max(lens) // page), tokens // page)
+        case = _attend_case(len(lens) + dim, dtype, dim, heads, heads_kv, page, lens, q_len=q_len, width=width)
+        _check_attend(case, page, q_len, _attend(case, page, q_len, dtype, is_causal=causal), causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch, width", [(40, 16), (40, 33), (300, 64), (300, 65), (300, 300)])
+def test_fp4_decode_of_ragged_batches_with_tables_of_few_and_of_many_tokens(batch, width):
+    require_gfx950()
+    rng = random.Random(batch + width)
+    lens = [rng.choice([0, 1, 16 * rng.randint(0, min(width, 64)), rng.randint(0, 256)]) for _ in range(batch)]
+    case = _attend_case(batch, BF16, 64, 4, 2, 16, lens, width=width)
+    _check_attend(case, 16, 1, _attend(case, 16, 1, BF16))
+
+
+@pytest.mark.gpu
 def test_fp4_decode_rows_do_not_see_what_is_masked():
     """NaN blocks in tokens that only later queries see leave the earlier queries' rows alone, and reach the later ones."""
     require_gfx950()

@@ -8,7 +8,8 @@
 //    128-token unit of every sequence, in batch order -- is cut into n_parts equal ranges on the device, so that compute
 //    units get the same number of units whatever the lengths are and nothing is read back.  The waves take the 32-token
 //    tiles of a unit in turn and meet once per sequence, in LDS.  A sequence that lies in one range is written out there;
-//    the others leave normalised fp32 rows with log-sum-exps for the merge kernel.
+//    the others leave normalised fp32 rows with log-sum-exps for the merge kernel.  Where the block tables address few tokens
+//    a range is a sequence: nothing is left to merge.
 //  * Q.K^T: v_mfma_scale_f32_16x16x128_f8f6f4 with the K codes as they lie in memory -- lane (c, g) supplies block g of token
 //    c, sixteen bytes, and its scale byte -- against the query row as a sum of two (bf16: exact) or three (fp16: exact) e4m3 rows.
 //    Tokens sit on the M axis, so every softmax quantity of a query row is local to a lane column.
@@ -45,6 +46,7 @@ struct Fp4Params {
   float *part_o, *part_lse;
   int batch, q_len, heads, heads_kv, page_size, group, rows, row_groups, n_parts, max_len, causal, negate_q;
   int n_pages;
+  int by_sequence;  // part i is sequence i (tables of few tokens), with nothing to merge
   float score_scale, cap_log2e;  // scale of a score to its logit2, with a cap to 2 log2(e) times the tanh's argument
 };
 
@@ -145,39 +147,55 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     const int len = len_of(p, min(base + lane, p.batch - 1));
     return base + lane < p.batch ? len : 0;
   };
-  for (int base = 0; base < p.batch; base += 64) {
-    const int len = read_lens(base), n = units_of_len(len), incl = wave_incl_scan(n);
-    if (base == 0) {
-      lens = len;
-      n0 = n;
-      incl0 = incl;
+  const int row0 = rg * 16 * NRB;
+  int u_begin, u_end, b_first = -1, pre_first = 0;
+  if (p.by_sequence) {
+    lens = read_lens(part);
+    lens_base = part;
+    u_begin = 0;
+    u_end = units_of_len(uni(__builtin_amdgcn_readlane(lens, 0)));
+    b_first = part;
+    if (u_end == 0) {
+      for (int i = threadIdx.x; i < min(16 * NRB, p.rows - row0) * (D / 8); i += 64 * kWaves) {
+        const int r = row0 + i / (D / 8), s = r / p.group, gi = r - s * p.group;
+        *(u32x4*)(p.out + (((int64_t)part * p.q_len + s) * p.heads + kvh * p.group + gi) * D + 8 * (i % (D / 8))) = u32x4{0, 0, 0, 0};
+      }
+      return;
     }
-    T += __builtin_amdgcn_readlane(incl, 63);
-  }
-  T = uni(T);
-  if (T == 0) return;
-  const Ranges ranges(T, p.n_parts);
-  if (part >= (int)ranges.np) return;
-  const int u_begin = uni(ranges.begin(part)), u_end = uni(ranges.begin(part + 1));
-  int b_first = -1, pre_first = 0;
-  for (int base = 0, carry = 0; base < p.batch && b_first < 0; base += 64) {
-    int n = n0, incl = incl0;
-    if (base > 0) {
-      lens = read_lens(base);
-      lens_base = base;
-      n = units_of_len(lens);
-      incl = wave_incl_scan(n);
+  } else {
+    for (int base = 0; base < p.batch; base += 64) {
+      const int len = read_lens(base), n = units_of_len(len), incl = wave_incl_scan(n);
+      if (base == 0) {
+        lens = len;
+        n0 = n;
+        incl0 = incl;
+      }
+      T += __builtin_amdgcn_readlane(incl, 63);
     }
-    const uint64_t hit = __ballot(carry + incl > u_begin);
-    if (hit) {
-      const int at = uni(__ffsll((unsigned long long)hit) - 1);
-      b_first = base + at;
-      pre_first = carry + __builtin_amdgcn_readlane(incl - n, at);
+    T = uni(T);
+    if (T == 0) return;
+    const Ranges ranges(T, p.n_parts);
+    if (part >= (int)ranges.np) return;
+    u_begin = uni(ranges.begin(part));
+    u_end = uni(ranges.begin(part + 1));
+    for (int base = 0, carry = 0; base < p.batch && b_first < 0; base += 64) {
+      int n = n0, incl = incl0;
+      if (base > 0) {
+        lens = read_lens(base);
+        lens_base = base;
+        n = units_of_len(lens);
+        incl = wave_incl_scan(n);
+      }
+      const uint64_t hit = __ballot(carry + incl > u_begin);
+      if (hit) {
+        const int at = uni(__ffsll((unsigned long long)hit) - 1);
+        b_first = base + at;
+        pre_first = carry + __builtin_amdgcn_readlane(incl - n, at);
+      }
+      carry += __builtin_amdgcn_readlane(incl, 63);
     }
-    carry += __builtin_amdgcn_readlane(incl, 63);
   }
 
-  const int row0 = rg * 16 * NRB;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
   const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f;
   const uint32_t q_sign = p.negate_q ? 0x80808080u : 0u;
@@ -794,6 +812,7 @@ const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_decode_fp4_kernel<QT, D, NRB, false>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return hipGetErrorString(e);
+  if (p.by_sequence) return nullptr;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
   if (rows_all * p.batch <= 8192)
     hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 1>), dim3((unsigned)((rows_all + 3) / 4), p.batch), dim3(256), 0, s, p);
@@ -855,6 +874,11 @@ const char* launch_decode_fp4(const void* q, const void* k, const void* v, const
   p.causal = causal;
   p.n_pages = (int)n_pages;
   const size_t slots = (size_t)2 * n_parts * heads_kv * p.rows;
+  // Tables of few tokens: a workgroup per (sequence, kv head, row group) and no merge.  64 query heads on 8, dim 128, ranges / whole: 1 x 384
+  // tokens 8.2 / 5.7 us, 1 x 1024 8.6 / 8.3, 1 x 2048 8.9 / 12.4; 32 x 2048 19.3 / 16.6, 32 x 4096 30.1 / 29.9; 128 of 1 .. 512 24 / 15,
+  // 128 of 1 .. 4096 62 / 68: up to eight units whatever the batch is, up to sixteen where it has work for half of the ranges' workgroups.
+  p.by_sequence = p.max_len <= (2 * (int64_t)batch >= n_parts ? 16 : 8) * kUnit;
+  if (p.by_sequence) p.n_parts = batch;
   p.part_o = (float*)workspace;
   p.part_lse = (float*)((char*)workspace + align256(slots * dim * sizeof(float)));
   // the kernel takes maxima before it scales: the sign of the scale goes into the query

@@ -569,7 +569,10 @@ def _attend(case, page, q_len, dtype, **kw):
 def _check_attend(case, page, q_len, out, sm_scale=None, softcap=0.0, causal=True):
     """Bound on an element's error: the output's rounding (half a step of its type), each probability's rounding to bf16 (2^-8; two
     parts with fp16 queries: 2^-16), the query's e4m3 parts (2^-17 of its largest element, times the sum of |k|, moves a logit by
-    dz and a normalised probability by a factor of 2 dz at most) and 2^-13 for the logits' and sums' own 32-bit roundings."""
+    dz and a normalised probability by a factor of 2 dz at most) and 2^-13 for the logits' and sums' own 32-bit roundings.
+    Numbers below 2^-126 may be taken as zero.  The kernel's probabilities are relative to a maximum that some seen token reaches or
+    exceeds, so their sum is at least 1 and such a probability, or its product with a value, moves the row by 2^-126 max(|v|, 1) at
+    most; the weights of the ranges that share a sequence, at most one per token, and their products likewise: 2^-124 max(|v|, 1) a token."""
     q, k, v, ks, vs, lens, table = case
     D = q.shape[-1]
     sm_scale = D ** -0.5 if sm_scale is None else sm_scale
@@ -577,6 +580,8 @@ def _check_attend(case, page, q_len, out, sm_scale=None, softcap=0.0, causal=Tru
     half_step = torch.finfo(q.dtype).eps / 2
     dz = 2.0 ** -17 * q.double().abs().amax(-1, keepdim=True) * reach * abs(sm_scale)
     bound = half_step * ref.abs() * 1.01 + ((2.0 ** -8 if q.dtype == BF16 else 2.0 ** -16) + 2 * dz + 2.0 ** -13) * spread + _subnormal(q.dtype)
+    largest = ref_fp4_values(v, vs).double().abs().nan_to_num(nan=1.0).max().clamp(min=1)
+    bound = bound + 2.0 ** -124 * lens.double().reshape(-1, 1, 1, 1) * largest
     off = (out.double() - ref).abs()
     assert bool((off <= bound).all()), f"largest excess {(off - bound).max().item()}, at {(off - bound).argmax().item()}"
 
@@ -616,6 +621,25 @@ def test_fp4_decode_scales_and_caps(kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(softcap=5.0), dict(softcap=30.0, sm_scale=-0.2), dict(sm_scale=0.0), dict(sm_scale=-0.3), dict(sm_scale=2.0)])
+def test_fp4_decode_scales_and_caps_with_wide_tables(kw):
+    require_gfx950()
+    for dim, q_len in ((128, 1), (64, 5), (128, 9)):
+        case = _attend_case(dim, BF16, dim, 8, 2, 16, [200, 37, 129], q_len=q_len, width=25000)
+        _check_attend(case, 16, q_len, _attend(case, 16, q_len, BF16, **kw), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, dim, heads, heads_kv, q_len", [(BF16, 128, 8, 1, 1), (FP16, 64, 2, 1, 1), (BF16, 256, 4, 4, 1), (BF16, 128, 16, 2, 4)])
+def test_fp4_decode_joins_many_ranges(dtype, dim, heads, heads_kv, q_len):
+    """Few sequences in many ranges, so that a workgroup joins a row's; one that lies in a single range and one without tokens beside it."""
+    require_gfx950()
+    for lens in ([9000], [5000, 0, 100], [256 * 17 + 1, 130]):
+        case = _attend_case(len(lens) + dim, dtype, dim, heads, heads_kv, 16, lens, q_len=q_len)
+        _check_attend(case, 16, q_len, _attend(case, 16, q_len, dtype))
+
+
+@pytest.mark.gpu
 def test_fp4_decode_over_many_sequences_and_ranges():
     """More sequences than lanes of a wave, more than the ranges of the stream, and one that every range has a part of."""
     require_gfx950()
@@ -633,7 +657,7 @@ def test_fp4_decode_over_many_sequences_and_ranges():
 def test_fp4_decode_with_tables_of_few_and_of_many_tokens(dtype, q_len, dim, heads, heads_kv, page, lens, causal):
     """The width of the tables, not the lengths, decides how the work is cut: both ways give the plain form's rows, at each border too."""
     require_gfx950()
-    units = {0, 8 * 128, 16 * 128, 40000}
+    units = {0, 8 * 128, 16 * 128, 40000, 400000}  # (the widest: two blocks of rows per wave where there are more than sixteen)
     for tokens in sorted(units | {u + page for u in units}):
         width = max(-(-max(lens) // page), tokens // page)
         case = _attend_case(len(lens) + dim, dtype, dim, heads, heads_kv, page, lens, q_len=q_len, width=width)
@@ -651,11 +675,12 @@ def test_fp4_decode_of_ragged_batches_with_tables_of_few_and_of_many_tokens(batc
 
 
 @pytest.mark.gpu
-def test_fp4_decode_rows_do_not_see_what_is_masked():
+@pytest.mark.parametrize("width", [None, 200, 25000])
+def test_fp4_decode_rows_do_not_see_what_is_masked(width):
     """NaN blocks in tokens that only later queries see leave the earlier queries' rows alone, and reach the later ones."""
     require_gfx950()
     q_len, page = 8, 16
-    case = _attend_case(77, BF16, 128, 4, 1, page, [200, 8, 31], q_len=q_len)
+    case = _attend_case(77, BF16, 128, 4, 1, page, [200, 8, 31], q_len=q_len, width=width)
     q, k, v, ks, vs, lens, table = case
     for which in (ks, vs):
         b, token = 0, 196  # seen by the queries 4..7

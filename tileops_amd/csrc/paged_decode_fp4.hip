@@ -17,6 +17,15 @@
 //    tokens -- those whose probabilities it holds already -- widens them with their scale (v_cvt_scalef32_pk_bf16_fp4) and pairs the
 //    tokens with byte permutes: V needs no LDS, P does not move.
 //  * K, V and scales go from memory to registers, a tile ahead of their use, across the borders of sequences.
+//
+// Roundings: the query's e4m3 rows add up to it exactly (fp16 elements far below their row's largest excepted: 2^-17 of that one); a
+// probability becomes one bf16 (two for fp16 queries, whose rows carry three bits more), because PV then runs at the rate of 16-bit
+// products, and the row's sum is formed of the rounded ones, so that a common error cancels.  All else is fp32.
+//
+// Bound and measured (64 query heads on 8 kv heads, dim 128): 8 x 131072 tokens, 1.14 GB in 178 us, 6.4 TB/s: memory.  64 sequences of
+// 1024 .. 16384 tokens, 304 MB in 48 us.  32 sequences of as many with eight query tokens and capped scores: 311 MB in 128 us, bound by
+// the vector unit -- per tile of 32 tokens and two row blocks about 270 vector instructions, 48 of them exponentials and reciprocals at
+// half rate, beside 26 matrix instructions.  One sequence of 300 tokens: 5.5 us, the chain of loads length, table entry, tile.
 #include <climits>
 #include <type_traits>
 
@@ -46,6 +55,7 @@ struct Fp4Params {
   float *part_o, *part_lse;
   int batch, q_len, heads, heads_kv, page_size, group, rows, row_groups, n_parts, max_len, causal, negate_q;
   int n_pages;
+  int range_units;  // that a range has at least, where there are as many
   int by_sequence;  // part i is sequence i (tables of few tokens), with nothing to merge
   float score_scale, cap_log2e;  // scale of a score to its logit2, with a cap to 2 log2(e) times the tanh's argument
 };
@@ -53,12 +63,12 @@ struct Fp4Params {
 __device__ __forceinline__ int len_of(const Fp4Params& p, int b) { return min(max(p.seqlens[b], 0), p.max_len); }
 __device__ __forceinline__ int units_of_len(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
 
-// The T units cut into NP = min(n_parts, T) ranges, none of them empty, with bounds floor(p * T / NP) = p * (T / NP) +
+// The T > 0 units cut into NP = min(n_parts, ceil(T / range_units)) ranges, none of them empty, with bounds floor(p * T / NP) = p * (T / NP) +
 // floor(p * (T % NP) / NP); NP <= 4096 keeps the second product below 2^24.
 struct Ranges {
   uint32_t np, tq, tr;
-  __device__ __forceinline__ Ranges(int t, int n_parts) {
-    np = (uint32_t)max(min(n_parts, t), 1);
+  __device__ __forceinline__ Ranges(int t, const Fp4Params& p) {
+    np = (uint32_t)min(p.n_parts, 1 + (t - 1) / p.range_units);  // (t > 0)
     tq = (uint32_t)t / np;
     tr = (uint32_t)t % np;
   }
@@ -110,13 +120,15 @@ template <int SEL> __device__ __forceinline__ uint32_t widen2(uint32_t w, float 
 typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
 __device__ __forceinline__ int scalar_load(const int32_t* p, int i) { return ((scalar_ptr)(uintptr_t)p)[i]; }
 
-// Stream reads: a tile is read once per row group, and never again.
+// Stream reads: a tile is read once per row group, and never again (8 x 131072 tokens: 207 us through the caches, 191 past them).
 typedef const __attribute__((address_space(1))) uint8_t* global_ptr;
 template <typename T> __device__ __forceinline__ T stream_load(global_ptr p) {
   return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*)p);
 }
 
-// PT: a page holds whole tiles (its size is a multiple of kTile), else it holds whole blocks of sixteen tokens.
+// PT: a page holds whole tiles (its size is a multiple of kTile), else it holds whole blocks of sixteen tokens, each with a table entry
+// and addresses of its own (pages of 64, whole tiles / blocks: 32 x 4096 tokens at dim 64 26.4 / 27.1 us, 8 x 4096 with eight query tokens
+// at dim 128 28.9 / 29.6, else within 1%).
 template <typename QT, int D, int NRB, bool PT>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const Fp4Params p) {
   constexpr bool F16 = __is_same(QT, fp16_tag);
@@ -174,7 +186,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     }
     T = uni(T);
     if (T == 0) return;
-    const Ranges ranges(T, p.n_parts);
+    const Ranges ranges(T, p);
     if (part >= (int)ranges.np) return;
     u_begin = uni(ranges.begin(part));
     u_end = uni(ranges.begin(part + 1));
@@ -702,14 +714,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   }
 }
 
-// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  One wave takes R rows
-// (four where there are tens of thousands, so that they are one round of waves); a lane has four head elements, so the 64 / (D / 4)
+// Rows of a sequence that several ranges share: weights exp2(lse - max) over the ranges' normalised rows.  A lane has four head elements, so the 64 / (D / 4)
 // lane groups of a wave take different ranges.  All rows' first loads are in flight before the first weight is known.  Sequences
 // without tokens get zeros here.
-template <typename QT, int D, int R, int PRE>
-__device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t row0, int64_t rows_all, int first, int n, bool second) {
+// SHARED: the four waves of a workgroup take a quarter of a row's ranges each and join in LDS.
+// Bound: latency (a few MB in 3 to 7 us).
+template <int D> struct MergeShared {
+  float o[kWaves][D], m[kWaves], w[kWaves];
+};
+template <typename QT, int D, int R, int PRE, bool SHARED>
+__device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t row0, int64_t rows_all, int first, int n, bool second, MergeShared<D>* sh) {
   constexpr int LPR = D / 4, GROUPS = 64 / LPR;  // lanes per row, ranges side by side; PRE: loads of a row in flight
-  const int lane = threadIdx.x & 63, grp = lane / LPR, d0 = 4 * (lane % LPR);
+  static_assert(!SHARED || R == 1, "a shared row");
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), grp = lane / LPR, d0 = 4 * (lane % LPR);
+  const int share = SHARED ? (n + kWaves - 1) / kWaves : n, begin = SHARED ? min(wave * share, n) : 0, end = SHARED ? min(begin + share, n) : n;
   auto slot_of = [&](int i, int64_t row) __attribute__((always_inline)) -> int64_t {
     const int k = min(i, n - 1);
     return (int64_t)(2 * (first + k) + (k == 0 && second ? 1 : 0)) * rows_all + row;
@@ -722,7 +740,7 @@ __device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t ro
     M[r] = -INFINITY;
     W[r] = 0.f;
   }
-  for (int base = 0; base < n; base += PRE * GROUPS) {
+  for (int base = begin; base < end; base += PRE * GROUPS) {
     f32x4 x[R][PRE];
     float lse[R];
 #pragma unroll
@@ -730,7 +748,7 @@ __device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t ro
       const int64_t row = row0 + r < rows_all ? row0 + r : rows_all - 1;
 #pragma unroll
       for (int i = 0; i < PRE; i++) x[r][i] = *(const f32x4*)(p.part_o + slot_of(base + i * GROUPS + grp, row) * D + d0);
-      lse[r] = lane < PRE * GROUPS && base + lane < n ? p.part_lse[slot_of(base + lane, row)] : -INFINITY;
+      lse[r] = lane < PRE * GROUPS && base + lane < end ? p.part_lse[slot_of(base + lane, row)] : -INFINITY;
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -760,6 +778,29 @@ __device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t ro
       for (int e = 0; e < 4; e++) acc[r][e] += __shfl_xor(acc[r][e], m, 64);
     }
     const int64_t row = row0 + r;
+    if constexpr (SHARED) {
+      if (grp == 0) *(f32x4*)&sh->o[wave][d0] = acc[0];
+      if (lane == 0) {
+        sh->m[wave] = M[0];
+        sh->w[wave] = W[0];
+      }
+      __syncthreads();
+      if (wave > 0) return;
+      float top = M[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) top = fmaxf(top, sh->m[w]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      acc[0] = f32x4{0.f, 0.f, 0.f, 0.f};
+      W[0] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float f = fast_exp2(sh->m[w] - ref);
+        if (f != 0.f) {  // (no range, or none with a weight)
+          W[0] += f * sh->w[w];
+          acc[0] += f * *(const f32x4*)&sh->o[w][d0];
+        }
+      }
+    }
     if (grp > 0 || row >= rows_all) continue;
     const float inv = W[r] == 0.f ? 0.f : 1.0f / W[r];
     const int kvh = (int)(row / p.rows), qr = (int)(row - (int64_t)kvh * p.rows), s = qr / p.group, gi = qr - s * p.group;
@@ -768,38 +809,46 @@ __device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t ro
   }
 }
 
+// R rows of a wave; R = 0: a row of a workgroup.
 template <typename QT, int D, int R>
-__global__ __launch_bounds__(256) void paged_decode_fp4_merge_kernel(const Fp4Params p) {
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_fp4_merge_kernel(const Fp4Params p) {
+  __shared__ __attribute__((aligned(16))) MergeShared<D> sh[1];
   const int b = blockIdx.y;
-  const int64_t rows_all = (int64_t)p.heads_kv * p.rows, row0 = ((int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6)) * R;
+  const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
+  const int64_t row0 = R == 0 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * kWaves + uni(threadIdx.x >> 6)) * R;
   int pre;
   const int T = total_units(p, b, &pre);
   const int nu = uni(units_of_len(len_of(p, b)));
   int first = 0, last = -1;
   bool second = false;
   if (nu > 0) {
-    const Ranges ranges(T, p.n_parts);
+    const Ranges ranges(T, p);
     first = uni(ranges.owner(pre));
     last = uni(ranges.owner(pre + nu - 1));
     if (first == last) return;  // written by the range that holds it
     second = ranges.begin(first) != pre;
   }
-  if (row0 >= rows_all) return;
   const int n = last - first + 1;
   constexpr int GROUPS = 256 / D;
-  if (n <= 2 * GROUPS) {
-    merge_rows<QT, D, R, 2>(p, b, row0, rows_all, first, n, second);
+  if constexpr (R == 0) {
+    if (n <= 2 * GROUPS * kWaves) merge_rows<QT, D, 1, 2, true>(p, b, row0, rows_all, first, n, second, sh);
+    else merge_rows<QT, D, 1, 8, true>(p, b, row0, rows_all, first, n, second, sh);
   } else {
-    for (int r = 0; r < R && row0 + r < rows_all; r++) merge_rows<QT, D, 1, 8>(p, b, row0 + r, rows_all, first, n, second);
+    if (row0 >= rows_all) return;
+    if (n <= 2 * GROUPS) {
+      merge_rows<QT, D, R, 2, false>(p, b, row0, rows_all, first, n, second, nullptr);
+    } else {
+      for (int r = 0; r < R && row0 + r < rows_all; r++) merge_rows<QT, D, 1, 8, false>(p, b, row0 + r, rows_all, first, n, second, nullptr);
+    }
   }
 }
 
 constexpr int kMaxParts4 = 4096;
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Blocks of sixteen query rows per wave (two at head dim 256 do not fit the register file).
+// Blocks of sixteen query rows per wave, for calls with much to read (two at head dim 256 do not fit the register file).
 int row_blocks(int rows, int dim) { return rows <= 16 || dim == 256 ? 1 : 2; }
-int row_groups_of(int rows, int dim) { return (rows + 16 * row_blocks(rows, dim) - 1) / (16 * row_blocks(rows, dim)); }
+int row_groups_of(int rows, int blocks) { return (rows + 16 * blocks - 1) / (16 * blocks); }
 
 template <typename QT, int D, int NRB>
 const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
@@ -814,7 +863,12 @@ const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
   if (e != hipSuccess) return hipGetErrorString(e);
   if (p.by_sequence) return nullptr;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
-  if (rows_all * p.batch <= 8192)
+  // Few rows have many ranges each: a workgroup per row; many rows are one round of waves with four rows each.  Whole call, wave per row / workgroup
+  // per row: 64 rows of 16384 tokens 14.3 / 11.9 us, 256 rows 19.3 / 19.3, 512 rows 22.7 / 24.0; one row / four rows of a wave: 512 rows 31.3 / 35.2,
+  // 4096 rows 52.1 / 52.8, 8192 rows 98.5 / 97.7, 32768 rows 117.7 / 111.5.
+  if (rows_all * p.batch <= 256)
+    hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 0>), dim3((unsigned)rows_all, p.batch), dim3(256), 0, s, p);
+  else if (rows_all * p.batch < 8192)
     hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 1>), dim3((unsigned)((rows_all + 3) / 4), p.batch), dim3(256), 0, s, p);
   else
     hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<QT, D, 4>), dim3((unsigned)((rows_all + 15) / 16), p.batch), dim3(256), 0, s, p);
@@ -823,8 +877,8 @@ const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
 }
 
 template <typename QT>
-const char* launch_fp4_dim(const Fp4Params& p, int dim, hipStream_t s) {
-  const bool one = row_blocks(p.rows, dim) == 1;
+const char* launch_fp4_dim(const Fp4Params& p, int dim, int blocks, hipStream_t s) {
+  const bool one = blocks == 1;
   if (dim == 64) return one ? launch_fp4<QT, 64, 1>(p, s) : launch_fp4<QT, 64, 2>(p, s);
   if (dim == 128) return one ? launch_fp4<QT, 128, 1>(p, s) : launch_fp4<QT, 128, 2>(p, s);
   return launch_fp4<QT, 256, 1>(p, s);
@@ -832,9 +886,10 @@ const char* launch_fp4_dim(const Fp4Params& p, int dim, hipStream_t s) {
 
 }  // namespace
 
-// Ranges of the token stream: two workgroups (eight waves) per compute unit, over all (kv head, row group) pairs.
+// Ranges of the token stream: two workgroups (eight waves) per compute unit, over all (kv head, row group) pairs (8 x 131072 tokens: two 191 us,
+// three 218).
 int fp4_num_parts(int heads_kv, int rows, int dim, int compute_units) {
-  const int64_t parts = 2 * (int64_t)compute_units / ((int64_t)heads_kv * row_groups_of(rows, dim));
+  const int64_t parts = 2 * (int64_t)compute_units / ((int64_t)heads_kv * row_groups_of(rows, row_blocks(rows, dim)));
   return parts < 1 ? 1 : parts > kMaxParts4 ? kMaxParts4 : (int)parts;
 }
 
@@ -868,11 +923,21 @@ const char* launch_decode_fp4(const void* q, const void* k, const void* v, const
   p.page_size = page_size;
   p.group = heads / heads_kv;
   p.rows = q_len * p.group;
-  p.row_groups = row_groups_of(p.rows, dim);
-  p.n_parts = n_parts;
+  // What a range adds to the merge grows with the rows.  2 x 3000 tokens of 8 rows on 8 kv heads, ranges of 1 / 2 / 4 units: 10.7 / 9.6 /
+  // 10.4 us, 1 x 4096 9.4 / 9.3 / 10.3; 4 x 4096 of 64 rows on 4: 20.2 / 20.8 / 17.7, 1 x 8192 of 64 rows on 8: 21.4 / 21.3 / 16.6.
+  p.range_units = p.rows < 32 ? 2 : 4;
   p.max_len = max_len < INT_MAX - kUnit ? max_len : INT_MAX - kUnit;
   p.causal = causal;
   p.n_pages = (int)n_pages;
+  // Two row blocks share what a wave does for K and V; one makes twice the workgroups, which calls with little to read need more.  64 rows on 8
+  // kv heads, one / two blocks: 1 x 4096 tokens 11.6 / 14.3 us, 4 x 3000 16.3 / 20.9, 4 x 8192 26.0 / 28.0, 4 x 16384 40.7 / 39.4, 32 x 16384
+  // 290 / 192; 24 rows on 4 kv heads: 4 x 4096 13.5 / 13.8, 32 x 4096 29.6 / 28.5.
+  const int most_blocks = row_blocks(p.rows, dim);
+  const int blocks = fp4_max_units(batch, p.max_len) * heads_kv <= 2048 ? 1 : most_blocks;
+  p.row_groups = row_groups_of(p.rows, blocks);
+  const int fewest_groups = row_groups_of(p.rows, most_blocks);
+  if (p.row_groups > fewest_groups) n_parts = n_parts * fewest_groups / p.row_groups > 1 ? n_parts * fewest_groups / p.row_groups : 1;
+  p.n_parts = n_parts;
   const size_t slots = (size_t)2 * n_parts * heads_kv * p.rows;
   // Tables of few tokens: a workgroup per (sequence, kv head, row group) and no merge.  64 query heads on 8, dim 128, ranges / whole: 1 x 384
   // tokens 8.2 / 5.7 us, 1 x 1024 8.6 / 8.3, 1 x 2048 8.9 / 12.4; 32 x 2048 19.3 / 16.6, 32 x 4096 30.1 / 29.9; 128 of 1 .. 512 24 / 15,
@@ -886,7 +951,7 @@ const char* launch_decode_fp4(const void* q, const void* k, const void* v, const
   sm_scale = fabsf(sm_scale);
   p.score_scale = softcap > 0.f ? 2.f * kLog2e * (sm_scale / softcap) : sm_scale * kLog2e;
   p.cap_log2e = softcap * kLog2e;
-  return q_dtype == MI355_DT_BF16 ? launch_fp4_dim<bf16_tag>(p, dim, s) : launch_fp4_dim<fp16_tag>(p, dim, s);
+  return q_dtype == MI355_DT_BF16 ? launch_fp4_dim<bf16_tag>(p, dim, blocks, s) : launch_fp4_dim<fp16_tag>(p, dim, blocks, s);
 }
 
 }  // namespace mi355

@@ -1052,3 +1052,26 @@ def test_another_kernel_class_is_not_passed_by():
 
     op.kernel_map[key] = Mine
     assert torch.equal(op(*args), want + 1)
+
+
+@pytest.mark.gpu
+def test_native_host_calls_in_inference_mode_and_small_outputs_of_one_allocation():
+    """Outputs of the bookkeeping calls lie side by side: each is writable by itself, and lives as long as it is held."""
+    require_gfx950()
+    for op, args, _ in _host_cases():
+        want = op(*[_clone(x) for x in args])
+        with torch.inference_mode():
+            got = op(*[_clone(x) for x in args])
+        assert all(torch.equal(a, b) for a, b in zip(_bytes(want), _bytes(got), strict=True)), type(op).__name__
+    op, args, _ = _host_cases()[1]
+    op(*[_clone(x) for x in args])
+    outs = op(*[_clone(x) for x in args])
+    kept = [t.clone() for t in outs]
+    for i, t in enumerate(outs):
+        assert t.is_contiguous() and t._version == 0 and not t.requires_grad
+        t.fill_(1)
+        assert all(torch.equal(u, k) for j, (u, k) in enumerate(zip(outs, kept)) if j > i), i
+    last = outs[-1]
+    del outs, t
+    junk = [torch.full((4096,), 7, dtype=torch.int32, device=DEV) for _ in range(50)]
+    assert last.tolist() == [1] and len(junk) == 50

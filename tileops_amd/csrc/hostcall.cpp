@@ -2,8 +2,8 @@
 //
 // A decode step's bookkeeping runs 3 to 6 us on the device; checks, allocations and argument conversions in the interpreter made the
 // host, not the device, set the pace of small steps.  Host time of a call, interpreter and operator registry / here: page allocation for
-// 64 sequences 16.8 / 7.5 us, release 12.8 / 5.7 us, append + rows read back 36.8 / 11.8 us, attention over 300 tokens 17.8 / 9.3 us
-// (which is what its two kernels take).
+// 64 sequences 16.8 / 5.9 us (7.5 with an allocation per output), release 12.8 / 5.5 us, append + rows read back 36.8 / 12 us, attention over
+// 300 tokens 17.8 / 6.3 us (less than its kernel takes).
 //
 // Every function here returns None when a call is not for it -- a tensor that is not a plain one on the current device, a gradient or a
 // dispatch mode in force, a check that does not hold -- and has then done nothing: the op's Python path takes the call and says what
@@ -18,6 +18,9 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <array>
+#include <utility>
 
 #include "../../include/mi355_tileops.h"
 
@@ -64,6 +67,23 @@ struct Call {
   }
   // The function behind at::empty on this device, without the dispatcher before it.
   Tensor empty(IntArrayRef shape, ScalarType type) const { return Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt)); }
+  // Several small outputs of a call in one allocation (each 64-byte aligned; freed with the last of them).
+  template <size_t N> std::array<Tensor, N> empties(const std::pair<int64_t, ScalarType> (&of)[N]) const {
+    int64_t at[N], bytes = 0;
+    for (size_t i = 0; i < N; i++) {
+      at[i] = bytes;
+      bytes += (of[i].first * (int64_t)c10::elementSize(of[i].second) + 63) / 64 * 64;
+    }
+    const Tensor block = empty({bytes}, ScalarType::Byte);
+    std::array<Tensor, N> out;
+    for (size_t i = 0; i < N; i++) {
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()), block.key_set(), c10::scalarTypeToTypeMeta(of[i].second));
+      c10::TensorImpl* t = out[i].unsafeGetTensorImpl();
+      t->set_storage_offset(at[i] / (int64_t)c10::elementSize(of[i].second));
+      t->set_sizes_contiguous({of[i].first});
+    }
+    return out;
+  }
   const Tensor* fail() {
     ok = false;
     return nullptr;
@@ -127,8 +147,8 @@ PyObject* kv_alloc(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *cached = c.dense(a[0], ScalarType::Int, {batch}), *list = c.dense(a[2], ScalarType::Int, {pages}),
                *count = c.dense(a[3], ScalarType::Int, {1}), *cu = c.optional(a[4], ScalarType::Int, {batch + 1});
   if (!c.ok) return none();
-  const Tensor slots = c.empty({total}, ScalarType::Long), positions = c.empty({total}, ScalarType::Int), lens = c.empty({batch}, ScalarType::Int),
-               refused = c.empty({batch}, ScalarType::Bool), left = c.empty({1}, ScalarType::Int);
+  const auto [slots, positions, lens, refused, left] = c.empties<5>(
+      {{total, ScalarType::Long}, {total, ScalarType::Int}, {batch, ScalarType::Int}, {batch, ScalarType::Bool}, {1, ScalarType::Int}});
   const int rc = mi355_kv_alloc((const int32_t*)ptr(cached), (const int32_t*)ptr(cu), (int32_t*)ptr(table), stride, (int)width, (const int32_t*)ptr(list),
                                 (const int32_t*)ptr(count), (int64_t*)slots.data_ptr(), (int32_t*)positions.data_ptr(), (int32_t*)lens.data_ptr(),
                                 (uint8_t*)refused.data_ptr(), (int32_t*)left.data_ptr(), (int)batch, (int)total, (int)page, (int)pages, (void*)stream);
@@ -150,7 +170,7 @@ PyObject* kv_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *finished = c.dense(a[0], ScalarType::Bool, {batch}), *lens = c.dense(a[1], ScalarType::Int, {batch}),
                *list = c.dense(a[3], ScalarType::Int, {pages}), *count = c.dense(a[4], ScalarType::Int, {1});
   if (!c.ok) return none();
-  const Tensor lens_out = c.empty({batch}, ScalarType::Int), count_out = c.empty({1}, ScalarType::Int);
+  const auto [lens_out, count_out] = c.empties<2>({{batch, ScalarType::Int}, {1, ScalarType::Int}});
   const int rc = mi355_kv_release((const uint8_t*)ptr(finished), (const int32_t*)ptr(lens), (const int32_t*)ptr(table), stride, (int)width, (int32_t*)ptr(list),
                                   (const int32_t*)ptr(count), (int32_t*)lens_out.data_ptr(), (int32_t*)count_out.data_ptr(), (int)batch, (int)page, (int)pages,
                                   (void*)stream);

@@ -22,10 +22,11 @@
 // probability becomes one bf16 (two for fp16 queries, whose rows carry three bits more), because PV then runs at the rate of 16-bit
 // products, and the row's sum is formed of the rounded ones, so that a common error cancels.  All else is fp32.
 //
-// Bound and measured (64 query heads on 8 kv heads, dim 128): 8 x 131072 tokens, 1.14 GB in 178 us, 6.4 TB/s: memory.  64 sequences of
-// 1024 .. 16384 tokens, 304 MB in 48 us.  32 sequences of as many with eight query tokens and capped scores: 311 MB in 128 us, bound by
-// the vector unit -- per tile of 32 tokens and two row blocks about 270 vector instructions, 48 of them exponentials and reciprocals at
-// half rate, beside 26 matrix instructions.  One sequence of 300 tokens: 5.5 us, the chain of loads length, table entry, tile.
+// Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
+// sequences of 512 .. 8192 tokens, 304 MB in 48 to 52 us, 5.8 to 6.3 TB/s: memory.  64 query heads, 32 sequences of 1024 .. 16384 tokens with
+// eight query tokens and capped scores: 311 MB in 125 to 140 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
+// 270 vector instructions, 48 of them exponentials and reciprocals at half rate, beside 26 matrix instructions.  One sequence of 300
+// tokens: 7.3 us, the chain of loads length, table entry, tile.
 #include <climits>
 #include <type_traits>
 

@@ -127,7 +127,7 @@ class PagedKVCacheAllocFwdOp(_ServingOp):
     ``total_q`` is the step's length, which may be padded behind the last sequence.  ``free_pages[:free_count]`` is a stack of free
     pages.  Sequences are served in batch order; one that would outgrow its row, or for which the pages do not last, is ``refused``: its
     ``real_seqlen_kv`` stays ``cache_seqlens[b]``, and its tokens -- like padding -- have slot and position -1.  ``free_count`` is not
-    written (a repeated call gives the same answer): pass ``free_count_out`` to the next step.
+    written (a repeated call gives the same answer): pass ``free_count_out`` to the next step.  The outputs may share one allocation.
     """
 
     _key = "paged_kv_cache_alloc_kernel"
@@ -180,7 +180,7 @@ class PagedKVCacheReleaseFwdOp(_ServingOp):
     ``forward(finished [batch] bool, seqlens [batch] int32, block_table [batch, max_pages_per_req] int32, free_pages [num_pages] int32,
     free_count [1] int32)`` writes the pages of the finished sequences' rows behind ``free_pages[:free_count]``, in batch order, and
     returns ``(seqlens_out, free_count_out)``: lengths with 0 for the finished, and the new count.  ``seqlens``, ``free_count`` and the
-    table are not written.
+    table are not written.  The outputs may share one allocation.
     """
 
     _key = "paged_kv_cache_release_kernel"

@@ -768,7 +768,7 @@ int mi355_kv_gather_fp4(const void* k_codes, const void* v_codes, const void* k_
   if (page_size <= 0) return fail(MI355_EINVAL, "page_size must be positive");
   if (n_phys_tokens <= 0 || n_phys_tokens % page_size != 0) return fail(MI355_EINVAL, "n_phys_tokens must be a positive multiple of page_size");
   if (!is_q_dtype(out_dtype)) return fail(MI355_EINVAL, "out_dtype must be bf16 or fp16, got code %d", out_dtype);
-  if ((int64_t)tokens * heads_kv * (dim / 8) / 256 >= INT_MAX) return fail(MI355_EUNSUPPORTED, "too many rows");
+  if ((int64_t)tokens * heads_kv * (dim / 8) > UINT32_MAX - 255) return fail(MI355_EUNSUPPORTED, "too many rows");
   if (tokens == 0) return MI355_OK;
   if (!k_codes || !v_codes || !k_scale || !v_scale || !slots || !k_out || !v_out) return fail(MI355_EINVAL, "null pointer argument");
   if (((uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)k_codes | (uintptr_t)v_codes) & 15)

@@ -534,7 +534,7 @@ template <typename XT, int CACHE, int KIND, typename R, int PASSES>
 __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
   const int lane = threadIdx.x & 63;
   const int lanes = p.dim >> 3, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
-  const int heads = KIND == kQuery ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^30: the launcher checks)
+  const int heads = KIND == kQuery ? p.heads : p.heads_kv, rows = p.tokens * heads;  // (below 2^26: the launcher checks)
   const int row0 = wave * PASSES * per_wave;
   if (row0 >= rows) return;
   const uint16_t* base = KIND == kQuery ? p.q : KIND == kKey ? p.k : p.v;
@@ -686,39 +686,53 @@ void launch_append_rows(const AppendParams& p, int cache, hipStream_t s) {
 }
 
 // --------------------------------------------------------------------------------------------- rows of the 4-bit cache
-// Eight elements per thread (four bytes of codes in, sixteen out).  Slots outside the pool give zeros.  Bound: memory (8192 tokens of 8 heads,
-// dim 128, 42 MB in 11.3 us, 3.7 TB/s; 64 tokens 2.9 us, the launch).
+// Eight elements of a key row and of its value row per thread (four bytes of codes in, sixteen out).  Slots outside the pool give zeros.
+// Bound: memory (8192 tokens of 8 heads, dim 128, 42 MB in 9.0 us, 4.7 TB/s, what a copy reaches; 64 tokens 2.9 us, the launch).
+struct GatherParams {
+  const uint8_t *codes[2], *scales[2];
+  const int64_t* slots;
+  u32x4* out[2];
+  uint32_t items, heads_kv;  // (items: threads, below 2^32 as in any grid)
+  int row_shift;             // log2 of the threads of a row, dim / 8
+  int page_size, page_shift; // log2 of page_size, -1 if it is no power of two
+  int64_t n_tokens;
+};
 template <typename XT>
-__global__ __launch_bounds__(256) void kv_gather_fp4_kernel(const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
-                                                            const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
-                                                            const int64_t* __restrict__ slots, uint4* __restrict__ k_out,
-                                                            uint4* __restrict__ v_out, int tokens, int heads_kv, int dim, int page_size,
-                                                            int64_t n_tokens) {
-  const int per_row = dim >> 3, per_token = heads_kv * per_row;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)tokens * per_token) return;
-  const int t = (int)(i / per_token), e = (int)(i - (int64_t)t * per_token), h = e / per_row, c = e - h * per_row;
-  const int64_t slot = slots[t];
-  uint4 r = {0, 0, 0, 0};
-  if (slot >= 0 && slot < n_tokens) {
-    const int64_t page = slot / page_size, row = (page * heads_kv + h) * page_size + (slot - page * page_size);
-    const uint32_t w = *(const uint32_t*)((blockIdx.y ? v : k) + row * (dim >> 1) + 4 * c);
-    const float sc = __uint_as_float((uint32_t)(blockIdx.y ? v_scale : k_scale)[row * (dim >> 5) + (c >> 2)] << 23);
+__global__ __launch_bounds__(256) void kv_gather_fp4_kernel(const GatherParams p) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= p.items) return;
+  const uint32_t row_of = i >> p.row_shift, c = i - (row_of << p.row_shift), t = row_of / p.heads_kv, h = row_of - t * p.heads_kv;
+  const int64_t slot = p.slots[t];
+  u32x4 r[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  if (slot >= 0 && slot < p.n_tokens) {
+    const int64_t page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+    const int64_t row = (page * p.heads_kv + h) * p.page_size + (slot - page * p.page_size);
+    uint32_t w[2], b[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      w[k] = *(const uint32_t*)(p.codes[k] + (row << (p.row_shift + 2)) + 4 * c);
+      b[k] = p.scales[k][(row << (p.row_shift - 2)) + (c >> 2)];
+    }
     typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
     typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-    if constexpr (__is_same(XT, bf16_tag)) {
-      r.x = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
-      r.y = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
-      r.z = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
-      r.w = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
-    } else {
-      r.x = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0));
-      r.y = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1));
-      r.z = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2));
-      r.w = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3));
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const float sc = __uint_as_float(b[k] << 23);
+      if constexpr (__is_same(XT, bf16_tag)) {
+        r[k][0] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[k], sc, 0));
+        r[k][1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[k], sc, 1));
+        r[k][2] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[k], sc, 2));
+        r[k][3] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[k], sc, 3));
+      } else {
+        r[k][0] = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[k], sc, 0));
+        r[k][1] = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[k], sc, 1));
+        r[k][2] = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[k], sc, 2));
+        r[k][3] = __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[k], sc, 3));
+      }
     }
   }
-  (blockIdx.y ? v_out : k_out)[i] = r;
+  p.out[0][i] = r[0];
+  p.out[1][i] = r[1];
 }
 
 const char* launched() {
@@ -799,13 +813,13 @@ const char* launch_qk_norm_rope_append(const void* q, const void* k, const void*
   const bool bf16 = x_dtype == MI355_DT_BF16;
   const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table | (uintptr_t)sin_table;
   const int64_t most_rows = (int64_t)tokens * (heads > heads_kv ? heads : heads_kv);
-  if (rotary_dim % (interleaved ? 8 : 16) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 30) &&
-      n_phys_tokens <= UINT32_MAX) {
+  if (rotary_dim % (interleaved ? 8 : 16) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 26)) {
     const bool many = append_passes(tokens, heads, heads_kv, 512 / dim) > 1;
     if (bf16) many ? launch_append_rows<bf16_tag, 4>(p, cache, s) : launch_append_rows<bf16_tag, 1>(p, cache, s);
     else many ? launch_append_rows<fp16_tag, 4>(p, cache, s) : launch_append_rows<fp16_tag, 1>(p, cache, s);
     return launched();
   }
+  if (tokens >= (1 << 24)) return "too many tokens for a grid";
   const dim3 grid(tokens, (heads + 2 * heads_kv + 3) / 4), block(256);
   auto kern = bf16 ? (cache == kCacheFp4 ? qk_norm_rope_append_kernel<bf16_tag, kCacheFp4>
                       : cache == kCacheFp8 ? qk_norm_rope_append_kernel<bf16_tag, kCacheFp8> : qk_norm_rope_append_kernel<bf16_tag, kCache16>)
@@ -819,10 +833,23 @@ const char* launch_kv_gather_fp4(const void* k, const void* v, const void* k_sca
                                  void* v_out, int tokens, int heads_kv, int dim, int page_size, int64_t n_phys_tokens, int out_dtype,
                                  hipStream_t s) {
   const int64_t items = (int64_t)tokens * heads_kv * (dim / 8);
-  const dim3 grid((unsigned)((items + 255) / 256), 2), block(256);
+  GatherParams p;
+  p.codes[0] = (const uint8_t*)k;
+  p.codes[1] = (const uint8_t*)v;
+  p.scales[0] = (const uint8_t*)k_scale;
+  p.scales[1] = (const uint8_t*)v_scale;
+  p.slots = slots;
+  p.out[0] = (u32x4*)k_out;
+  p.out[1] = (u32x4*)v_out;
+  p.items = (uint32_t)items;
+  p.heads_kv = (uint32_t)heads_kv;
+  p.row_shift = __builtin_ctz(dim / 8);  // (head dims 64, 128 and 256)
+  p.page_size = page_size;
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  p.n_tokens = n_phys_tokens;
+  const dim3 grid((unsigned)((items + 255) / 256)), block(256);
   auto kern = out_dtype == MI355_DT_BF16 ? kv_gather_fp4_kernel<bf16_tag> : kv_gather_fp4_kernel<fp16_tag>;
-  hipLaunchKernelGGL(kern, grid, block, 0, s, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_scale, (const uint8_t*)v_scale, slots,
-                     (uint4*)k_out, (uint4*)v_out, tokens, heads_kv, dim, page_size, n_phys_tokens);
+  hipLaunchKernelGGL(kern, grid, block, 0, s, p);
   return launched();
 }
 

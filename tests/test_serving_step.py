@@ -510,6 +510,75 @@ def test_append_of_values_that_are_not_numbers_and_of_the_largest():
 
 
 # ------------------------------------------------------------------------------------------------------ rows of the cache
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [FP4, FP8, None], ids=["fp4", "fp8", "16"])
+@pytest.mark.parametrize("dtype, dim, heads, heads_kv, tokens, rotary, interleaved, norm, weight_dtype", [
+    (BF16, 128, 14, 7, 1301, 128, False, True, None), (FP16, 64, 6, 2, 7001, 32, True, True, torch.float32), (BF16, 256, 6, 3, 1407, 256, False, False, None),
+    (BF16, 128, 12, 3, 9173, 96, False, True, torch.float32), (FP16, 256, 4, 1, 13661, 64, True, False, None), (BF16, 64, 5, 5, 22013, 0, False, True, None),
+], ids=str)
+def test_append_of_many_rows_equals_many_appends(cache, dtype, dim, heads, heads_kv, tokens, rotary, interleaved, norm, weight_dtype):
+    """A wave of a large call takes several rows in turn: each row's bits are those of small calls."""
+    require_gfx950()
+    page, g = 16, torch.Generator(device=DEV).manual_seed(dim + tokens)
+    qkv = torch.randn(tokens, (heads + 2 * heads_kv) * dim, generator=g, device=DEV).to(dtype)
+    q, k, v = (x.unflatten(1, (-1, dim)) for x in qkv.split([heads * dim, heads_kv * dim, heads_kv * dim], 1))
+    w = [torch.rand(dim, generator=g, device=DEV).to(weight_dtype or dtype) for _ in range(2)] if norm else [None, None]
+    tables = [torch.rand(500, rotary // 2, generator=g, device=DEV) for _ in range(2)] if rotary else [None, None]
+    positions = torch.randint(0, 500, (tokens,), generator=g, device=DEV, dtype=torch.int32) if rotary else None
+    pages = -(-tokens // page) + 2
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:tokens]
+    slots[tokens // 2] = -1
+    pools = [_append_args(cache, dim=dim, dtype=dtype, device=DEV, heads_kv=heads_kv, page=page, pages=pages) for _ in range(2)]
+    pools = [[a[n] for n in ("k_cache", "v_cache", "k_scale", "v_scale") if n in a] for a in pools]
+    op = AppendOp(heads, heads_kv, dim, page, rotary_dim=rotary, interleaved=interleaved, cache_dtype=cache)
+    out, parts = op(q, k, v, *w, *tables, positions, slots, *pools[0]), []
+    for i in range(0, tokens, 777):
+        n = slice(i, min(i + 777, tokens))
+        for m in (slice(n.start, (n.start + n.stop) // 2), slice((n.start + n.stop) // 2, n.stop)):
+            parts.append(op(q[m], k[m], v[m], *w, *tables, positions[m] if rotary else None, slots[m], *pools[1]))
+    assert torch.equal(out.view(torch.int16), torch.cat(parts).view(torch.int16))
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*pools))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [FP4, FP8, None], ids=["fp4", "fp8", "16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_leaves_what_is_not_rotated_as_it_is(cache, interleaved):
+    """Behind rotary_dim, without a norm: the very bits of queries and of 16-bit keys, infinities and zeros of either sign among them; with one,
+    a zero takes the weight's sign into its code."""
+    require_gfx950()
+    dim, rotary, tokens, heads, heads_kv, page = 128, 64, 6, 4, 2, 16
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v = (torch.randn(tokens, n, dim, generator=g, device=DEV).to(BF16) for n in (heads, heads_kv, heads_kv))
+    for x in (q, k, v):
+        x[:, :, 70], x[:, :, 71], x[:, :, 90] = 0.0, -0.0, -0.0
+    q[1, :, 100], q[2, :, 127] = float("inf"), float("-inf")
+    if cache is None:
+        k[1, 0, 64] = float("inf")
+    cos, sin = torch.rand(9, rotary // 2, generator=g, device=DEV), torch.rand(9, rotary // 2, generator=g, device=DEV)
+    positions, slots = _int([0, 3, 5, 8, 1, 2]), torch.tensor([3, 31, 0, 17, 9, 16], device=DEV)
+    a = _append_args(cache, device=DEV)
+    pools = [a[n] for n in ("k_cache", "v_cache", "k_scale", "v_scale") if n in a]
+    op = AppendOp(heads, heads_kv, dim, page, rotary_dim=rotary, interleaved=interleaved, cache_dtype=cache)
+    out = op(q, k, v, None, None, cos, sin, positions, slots, *pools)
+    bits = lambda x: x.contiguous().view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(out[..., rotary:]), bits(q[..., rotary:]))
+    if cache is None:
+        assert torch.equal(bits(pools[0][slots][..., rotary:]), bits(k[..., rotary:])) and torch.equal(bits(pools[1][slots]), bits(v))
+        return
+    weight = torch.full((dim,), -1.5, device=DEV)
+    for w, want in ((None, (0, 8, 8)), (weight, (8, 0, 0))):  # sign bits of the elements 70, 71 and 90
+        op(q, k, v, w, w, cos, sin, positions, slots, *pools)
+        for s in slots.tolist():
+            if cache == FP4:
+                row = pools[0][s // page, :, s % page].int()
+                got = [(row[:, 35] & 15).tolist(), (row[:, 35] >> 4).tolist(), (row[:, 45] & 15).tolist()]
+            else:
+                row = pools[0].view(torch.uint8)[s].int()
+                got = [(row[:, e] >> 4).tolist() for e in (70, 71, 90)]
+            assert got == [[x] * heads_kv for x in want], (w is None, s, got)
+
+
 def _random_cache(g, pages, heads_kv, page, dim, spread=6):
     codes = torch.randint(0, 256, (pages, heads_kv, page, dim // 2), generator=g, dtype=torch.uint8)
     scales = torch.randint(127 - spread, 127 + 1, (pages, heads_kv, page, dim // 32), generator=g, dtype=torch.uint8)

@@ -6,6 +6,7 @@
 // [n_pages, heads_kv, page_size, dim / 2], scales [n_pages, heads_kv, page_size, dim / 32]: the rows of one (page, kv head)
 // are contiguous, because a token-major pool would give every 64-byte row of a 128-byte line to another head's workgroup.
 #include <climits>
+#include <type_traits>
 
 #include "common.h"
 #include "device_utils.h"
@@ -364,8 +365,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendPa
 // lanes away: its raw elements come over as four dwords, and the lane norms them itself.  All rows of a wave are requested at its
 // start; tables are read again only when the token changes.
 // Takes: rotary_dim a multiple of 16 (interleaved: of 8), rows, tables and weights 16-byte aligned.
-// Bound: memory.  32 query heads on 8, dim 128, 4-bit cache: 8192 tokens in 52 us, 3.5 TB/s of what a copy reaches 4.7 (general form: 189 us),
-// 64 tokens in 4.0 us (5.0).
+// Bound: memory.  32 query heads on 8, dim 128, 4-bit cache: 8192 tokens in 44.5 us, 4.1 TB/s of what a copy reaches 4.7 (general form: 189 us),
+// 64 tokens in 3.7 us (5.0).  The kind of rotation is a template argument: its branches in the passes cost 7% (8192 tokens with four passes 52 us).
 // Four values (16-bit or fp32) of a weight or table as floats.
 template <typename XT>
 __device__ __forceinline__ f32x4 load_side4(const void* p, int64_t i, int fp32) {
@@ -413,21 +414,24 @@ __device__ __forceinline__ double inverse_root(double x) {  // the hardware's es
   return r * (1.5 - 0.5 * x * r * r);
 }
 
+enum { kNoTurn = 0, kHalves = 1, kPairs = 2 };  // rotation: none, of the two halves, of neighbouring pairs
+
 // Where a lane's eight elements stand in the rotation.
 struct Turn {
   bool on, upper;  // they are rotated; they are the second half of their pairs
-  int mate;        // lane of the row that holds the other half (its own if interleaved or not rotated)
+  int mate;        // lane of the row that holds the other half (its own for neighbouring pairs, or if they are not rotated)
 };
 
-// Coefficients of elements 4k .. 4k + 3 of the lane: y[e] = own[e] * c[e] + other[e] * s[e] with own, other normed rows.
-template <typename XT>
+// Coefficients of elements 4k .. 4k + 3 of the lane: y[e] = own[e] * c[e] + other[e] * s[e] with own, other normed rows.  Lanes that are not
+// rotated read the first coefficients and take 1 and -0 (with other = +0 the sum leaves every value as it is, zeros and infinities too).
+template <typename XT, int TURN>
 __device__ __forceinline__ void side4(const AppendParams& p, const Turn& t, int64_t tpos, int j, int k, f32x4* c, f32x4* s) {
   const int half = p.rotary_dim >> 1;
-  if (!t.on) {
+  if constexpr (TURN == kNoTurn) {
     *c = f32x4{1.f, 1.f, 1.f, 1.f};
     *s = f32x4{0.f, 0.f, 0.f, 0.f};
-  } else if (p.interleaved) {
-    const int64_t at = tpos * half + 4 * j + 2 * k;
+  } else if constexpr (TURN == kPairs) {
+    const int64_t at = tpos * half + (t.on ? 4 * j + 2 * k : 0);
     float c0, c1, s0, s1;
     if (p.table_fp32) {
       const f32x2 a = *(const f32x2*)((const float*)p.cos_table + at), b = *(const f32x2*)((const float*)p.sin_table + at);
@@ -442,10 +446,18 @@ __device__ __forceinline__ void side4(const AppendParams& p, const Turn& t, int6
     *c = f32x4{c0, c0, c1, c1};
     *s = f32x4{-s0, s0, -s1, s1};
   } else {
-    const int64_t at = tpos * half + 8 * j - (t.upper ? half : 0) + 4 * k;
+    const int64_t at = tpos * half + (t.on ? 8 * j - (t.upper ? half : 0) + 4 * k : 0);
     *c = load_side4<XT>(p.cos_table, at, p.table_fp32);
     *s = load_side4<XT>(p.sin_table, at, p.table_fp32);
-    if (!t.upper) *s = -*s;
+#pragma unroll
+    for (int e = 0; e < 4; e++) (*s)[e] = t.upper ? (*s)[e] : -(*s)[e];
+  }
+  if constexpr (TURN != kNoTurn) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      (*c)[e] = t.on ? (*c)[e] : 1.f;
+      (*s)[e] = t.on ? (*s)[e] : -0.f;
+    }
   }
 }
 
@@ -530,7 +542,7 @@ template <int PASSES> __device__ __forceinline__ void store_once(u32x4* p, u32x4
 }
 
 // Rows of one kind.  R: the type that norm and rotation are formed in (see the general form).
-template <typename XT, int CACHE, int KIND, typename R, int PASSES>
+template <typename XT, int CACHE, int KIND, typename R, int PASSES, int TURN>
 __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
   const int lane = threadIdx.x & 63;
   const int lanes = p.dim >> 3, j = lane & (lanes - 1), per_wave = 64 / lanes;  // lanes per row, the lane's place, rows per pass
@@ -540,12 +552,12 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
   const uint16_t* base = KIND == kQuery ? p.q : KIND == kKey ? p.k : p.v;
   const int64_t stride = KIND == kQuery ? p.q_stride : KIND == kKey ? p.k_stride : p.v_stride;
   const void* weight = KIND == kQuery ? p.q_weight : KIND == kKey ? p.k_weight : nullptr;
-  const bool rotates = KIND != kValue && p.rotary_dim > 0;
+  constexpr bool rotates = KIND != kValue && TURN != kNoTurn;
   const int apart = p.rotary_dim >> 4;  // lanes between the halves of a pair
   Turn turn;
   turn.on = rotates && 8 * j < p.rotary_dim;
   turn.upper = j >= apart;
-  turn.mate = turn.on && !p.interleaved ? (turn.upper ? j - apart : j + apart) : j;
+  turn.mate = turn.on && TURN == kHalves ? (turn.upper ? j - apart : j + apart) : j;
   const int mate_lane = lane - j + turn.mate;
 
   // the lane's rows, all requested at once: token and head, stepped instead of divided
@@ -584,10 +596,12 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
       w[k] = wo[k] = f32x4{1.f, 1.f, 1.f, 1.f};
       if (weight) {
         w[k] = load_side4<XT>(weight, 8 * j + 4 * k, p.weight_fp32);
-        wo[k] = p.interleaved ? f32x4{w[k][1], w[k][0], w[k][3], w[k][2]} : load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
+        wo[k] = TURN == kPairs ? f32x4{w[k][1], w[k][0], w[k][3], w[k][2]} : load_side4<XT>(weight, 8 * turn.mate + 4 * k, p.weight_fp32);
+#pragma unroll
+        for (int e = 0; e < 4; e++) wo[k][e] = turn.on ? wo[k][e] : 1.f;
       }
 #pragma unroll
-      for (int i = 0; i < (WIDE ? PASSES : 1); i++) side4<XT>(p, turn, tpos[i], j, k, &c[i][k], &s[i][k]);
+      for (int i = 0; i < (WIDE ? PASSES : 1); i++) side4<XT, TURN>(p, turn, tpos[i], j, k, &c[i][k], &s[i][k]);
       if constexpr (!WIDE) {
         c[0][k] *= w[k];
         s[0][k] *= wo[k];
@@ -605,32 +619,27 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
       Unpack<XT, 8>::run(x, y);
     } else {
       uint32_t other[4];
-      if (rotates) {
-        if (p.interleaved) {
+      if constexpr (rotates) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) other[e] = __builtin_amdgcn_alignbit(x[e], x[e], 16);  // the pair's elements changed over
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) other[e] = (uint32_t)__shfl((int)x[e], mate_lane, 64);
+        for (int e = 0; e < 4; e++) {
+          other[e] = TURN == kPairs ? __builtin_amdgcn_alignbit(x[e], x[e], 16) : (uint32_t)__shfl((int)x[e], mate_lane, 64);
+          other[e] = turn.on ? other[e] : 0u;
         }
       }
       float xf[8];
       Unpack<XT, 8>::run(x, xf);
-      R rstd = 1;
-      if (weight) {
-        R sum = 0;
+      R sum = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum += (R)xf[e] * (R)xf[e];
-        sum = over_row(sum, lanes, [](R a, R b) { return a + b; });
-        rstd = inverse_root(sum * inv_dim + (R)p.eps);
-      }
+      for (int e = 0; e < 8; e++) sum += (R)xf[e] * (R)xf[e];
+      sum = over_row(sum, lanes, [](R a, R b) { return a + b; });
+      const R root = inverse_root(sum * inv_dim + (R)p.eps), rstd = weight ? root : (R)1;
       float of[8];
-      if (rotates) Unpack<XT, 8>::run(other, of);
+      if constexpr (rotates) Unpack<XT, 8>::run(other, of);
       if constexpr (!WIDE) {
-        if (i > 0 && rotates && __ballot(t != tokens[i > 0 ? i - 1 : 0])) {  // another token's tables
+        if (rotates && i > 0 && __ballot(t != tokens[i > 0 ? i - 1 : 0])) {  // another token's tables
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            side4<XT>(p, turn, tpos[i], j, k, &c[0][k], &s[0][k]);
+            side4<XT, TURN>(p, turn, tpos[i], j, k, &c[0][k], &s[0][k]);
             c[0][k] *= w[k];
             s[0][k] *= wo[k];
           }
@@ -638,7 +647,7 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           float z = xf[e] * c[0][e >> 2][e & 3];
-          if (rotates) z = __builtin_fmaf(of[e], s[0][e >> 2][e & 3], z);
+          if constexpr (rotates) z = __builtin_fmaf(of[e], s[0][e >> 2][e & 3], z);
           y[e] = z * rstd;
         }
       } else {
@@ -646,7 +655,7 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
         for (int e = 0; e < 8; e++) {
           const int k = e >> 2, l = e & 3;
           R z = (R)xf[e] * (R)w[k][l] * (R)c[WIDE ? i : 0][k][l];
-          if (rotates) z += (R)of[e] * (R)wo[k][l] * (R)s[WIDE ? i : 0][k][l];
+          if constexpr (rotates) z += (R)of[e] * (R)wo[k][l] * (R)s[WIDE ? i : 0][k][l];
           y[e] = (float)(z * rstd);
         }
       }
@@ -661,27 +670,27 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, int wave) {
 }
 
 // PASSES of a wave over query rows; key and value rows, whose token changes more often, take half as many.
-template <typename XT, int CACHE, int PASSES>
+template <typename XT, int CACHE, int PASSES, int TURN>
 __global__ __launch_bounds__(256, 4) void qk_norm_rope_append_rows_kernel(const AppendParams p, int q_waves, int k_waves) {
   constexpr int KP = (PASSES + 1) / 2;
   int wave = blockIdx.x * 4 + uni(threadIdx.x >> 6);
   if (wave < k_waves) {  // (the longest rows first)
-    if constexpr (CACHE == kCache16) append_rows<XT, CACHE, kKey, float, KP>(p, wave);
-    else append_rows<XT, CACHE, kKey, double, KP>(p, wave);
+    if constexpr (CACHE == kCache16) append_rows<XT, CACHE, kKey, float, KP, TURN>(p, wave);
+    else append_rows<XT, CACHE, kKey, double, KP, TURN>(p, wave);
   } else if ((wave -= k_waves) < q_waves) {
-    append_rows<XT, CACHE, kQuery, float, PASSES>(p, wave);
+    append_rows<XT, CACHE, kQuery, float, PASSES, TURN>(p, wave);
   } else {
-    append_rows<XT, CACHE, kValue, float, KP>(p, wave - q_waves);
+    append_rows<XT, CACHE, kValue, float, KP, TURN>(p, wave - q_waves);
   }
 }
 
-template <typename XT, int PASSES>
+template <typename XT, int PASSES, int TURN>
 void launch_append_rows(const AppendParams& p, int cache, hipStream_t s) {
   auto waves = [&](int heads, int rows) { return (int)(((int64_t)p.tokens * heads + rows - 1) / rows); };
   const int q_waves = waves(p.heads, 512 / p.dim * PASSES), k_waves = waves(p.heads_kv, 512 / p.dim * ((PASSES + 1) / 2));
   const dim3 grid((q_waves + 2 * k_waves + 3) / 4), block(256);
-  auto kern = cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp4, PASSES>
-              : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp8, PASSES> : qk_norm_rope_append_rows_kernel<XT, kCache16, PASSES>;
+  auto kern = cache == kCacheFp4 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp4, PASSES, TURN>
+              : cache == kCacheFp8 ? qk_norm_rope_append_rows_kernel<XT, kCacheFp8, PASSES, TURN> : qk_norm_rope_append_rows_kernel<XT, kCache16, PASSES, TURN>;
   hipLaunchKernelGGL(kern, grid, block, 0, s, p, q_waves, k_waves);
 }
 
@@ -764,11 +773,12 @@ const char* launch_kv_release(const uint8_t* finished, const int32_t* seqlens, c
 }
 
 namespace {
-// Passes of a wave: one while that leaves a few waves per SIMD, four (all rows requested ahead) beyond.  32 query heads on 8, dim 128, 4-bit cache,
-// one / four passes: 256 tokens 4.6 / 5.4 us, 512 5.6 / 6.4, 1024 9.4 / 8.1, 2048 16.7 / 14.0, 8192 57 / 52 (FP8 and 16-bit caches alike).
+// Passes of a wave: one while that leaves a few waves per SIMD, then four, six in the largest calls (all rows of a wave are requested ahead).
+// 32 query heads on 8, dim 128, 4-bit cache, one / four / six passes: 256 tokens 4.3 / 4.8 us, 512 5.5 / 5.6, 1024 8.9 / 7.6 / 8.1, 2048
+// 15.6 / 12.9 / 13.0, 4096 27.7 / 23.8 / 23.1, 8192 51.5 / 48.5 / 44.1 (FP8 and 16-bit caches alike; 2050 tokens of 20 heads, dim 256, 10.5 / 11.4).
 int append_passes(int tokens, int heads, int heads_kv, int per_wave) {
   const int64_t passes = (int64_t)tokens * (heads + 2 * heads_kv) / per_wave;
-  return passes < 8192 ? 1 : 4;
+  return passes < 8192 ? 1 : passes < 40960 ? 4 : 6;
 }
 }  // namespace
 
@@ -814,9 +824,21 @@ const char* launch_qk_norm_rope_append(const void* q, const void* k, const void*
   const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table | (uintptr_t)sin_table;
   const int64_t most_rows = (int64_t)tokens * (heads > heads_kv ? heads : heads_kv);
   if (rotary_dim % (interleaved ? 8 : 16) == 0 && (bases & 15) == 0 && ((q_stride | k_stride | v_stride) & 7) == 0 && most_rows < (1 << 26)) {
-    const bool many = append_passes(tokens, heads, heads_kv, 512 / dim) > 1;
-    if (bf16) many ? launch_append_rows<bf16_tag, 4>(p, cache, s) : launch_append_rows<bf16_tag, 1>(p, cache, s);
-    else many ? launch_append_rows<fp16_tag, 4>(p, cache, s) : launch_append_rows<fp16_tag, 1>(p, cache, s);
+    const int passes = append_passes(tokens, heads, heads_kv, 512 / dim);
+    auto launch = [&](auto x_tag, auto turn) {
+      using XT = decltype(x_tag);
+      constexpr int TURN = decltype(turn)::value;
+      if (passes == 6) launch_append_rows<XT, 6, TURN>(p, cache, s);
+      else if (passes == 4) launch_append_rows<XT, 4, TURN>(p, cache, s);
+      else launch_append_rows<XT, 1, TURN>(p, cache, s);
+    };
+    auto launch_turn = [&](auto x_tag) {
+      if (rotary_dim == 0) launch(x_tag, std::integral_constant<int, kNoTurn>{});
+      else if (interleaved) launch(x_tag, std::integral_constant<int, kPairs>{});
+      else launch(x_tag, std::integral_constant<int, kHalves>{});
+    };
+    if (bf16) launch_turn(bf16_tag{});
+    else launch_turn(fp16_tag{});
     return launched();
   }
   if (tokens >= (1 << 24)) return "too many tokens for a grid";

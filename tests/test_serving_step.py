@@ -699,6 +699,17 @@ def test_fp4_decode_scales_and_caps_with_wide_tables(kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [2000.0, 3000.5, 1e5, 1e7])
+@pytest.mark.parametrize("width", [None, 25000])
+def test_fp4_decode_with_a_cap_far_above_the_scores(softcap, width):
+    """Scores of some tens under a cap of up to 1e7: a cap formed as cap - 2 cap / (exp(2x) + 1) in 32 bits would be off by 2^-24 of it."""
+    require_gfx950()
+    for dim, q_len, dtype in ((128, 1, BF16), (64, 5, FP16)):
+        case = _attend_case(dim, dtype, dim, 8, 2, 16, [200, 37, 129], q_len=q_len, width=width)
+        _check_attend(case, 16, q_len, _attend(case, 16, q_len, dtype, softcap=softcap, sm_scale=0.05), softcap=softcap, sm_scale=0.05)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, dim, heads, heads_kv, q_len", [(BF16, 128, 8, 1, 1), (FP16, 64, 2, 1, 1), (BF16, 256, 4, 4, 1), (BF16, 128, 16, 2, 4)])
 def test_fp4_decode_joins_many_ranges(dtype, dim, heads, heads_kv, q_len):
     """Few sequences in many ranges, so that a workgroup joins a row's; one that lies in a single range and one without tokens beside it."""

@@ -46,6 +46,7 @@ constexpr int kTile = 32;             // tokens per step of a wave
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kUnit = kTile * kWaves; // tokens per unit of the token stream
 constexpr float kRescaleGap4 = 8.0f;
+constexpr float kLargeCap = 4096.0f;  // of a cap in the log2 domain, see its use
 
 struct Fp4Params {
   const uint16_t* q;
@@ -129,7 +130,8 @@ template <typename T> __device__ __forceinline__ T stream_load(global_ptr p) {
 
 // PT: a page holds whole tiles (its size is a multiple of kTile), else it holds whole blocks of sixteen tokens, each with a table entry
 // and addresses of its own (pages of 64, whole tiles / blocks: 32 x 4096 tokens at dim 64 26.4 / 27.1 us, 8 x 4096 with eight query tokens
-// at dim 128 28.9 / 29.6, else within 1%).
+// at dim 128 28.9 / 29.6, else within 1%).  Caps far above any score are served by the latter only, so that the code for them is not in the way
+// of the others (which it cost 3%).
 template <typename QT, int D, int NRB, bool PT>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const Fp4Params p) {
   constexpr bool F16 = __is_same(QT, fp16_tag);
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   }
 
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
-  const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f;
+  const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f, large_cap = p.cap_log2e > kLargeCap;
   const uint32_t q_sign = p.negate_q ? 0x80808080u : 0u;
   // byte of the lane's block in a word of V scales (head dim 64: of the first of the word's two tokens), turned right by this
   // many bits, sits in a float's exponent
@@ -475,10 +477,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     }
     constexpr uint32_t kOnes = 0x3f803f80u;  // two bf16 ones
 
-    // scale of token 4g + j of block i for the lane's head elements: its byte turned to a float's exponent (255 reads as NaN)
+    // scale of token 4g + j of block i for the lane's head elements: its byte turned to a float's exponent, all that the conversion
+    // reads of it (255 is NaN); the bits beside it are other scales
     auto v_scale = [&](int i, int j) __attribute__((always_inline)) -> uint32_t {
       const uint32_t w = D == 64 ? vsr[i][j >> 1] : D == 128 ? vsr[i][j] : c & 8 ? vsr[i][NS > 4 ? 2 * j + 1 : 0] : vsr[i][NS > 4 ? 2 * j : 0];
-      return __builtin_amdgcn_alignbit(w, w, D == 64 && (j & 1) ? (v_turn + 16) & 31 : v_turn) & 0x7f800000u;
+      return __builtin_amdgcn_alignbit(w, w, D == 64 && (j & 1) ? (v_turn + 16) & 31 : v_turn);
     };
     // A operands of the PV product for two head elements at a time: word_of(j, w) is the pair w of token j (0..7) as two bf16
     auto value_operands = [&](auto word_of, auto use) __attribute__((always_inline)) {
@@ -526,7 +529,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       uint32_t pw[NRB][NB / 2][NP][4], seen_bits[NRB][NB / 2];
       float slope[NRB], offset[NRB], top[NRB];  // logit = slope * s + offset, slope >= 0 (the sign of the softmax scale is in the query)
       bool grown = false;
-      if (softcap) {
+      bool capped = false;
+      if constexpr (MASKED && !PT) {
+        if (large_cap) {
+          // the form below loses a large cap's 24th bit, which is too much of a score far below it: s becomes tanh(x), by its series for small
+          // x (x^9 / 46 left out: 4e-7 of it)
+          capped = true;
+#pragma unroll
+          for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+            for (int e = 0; e < 4 * NB; e++) {
+              const float a = s[rb][e >> 2][e & 3] * q_scale[rb], x = a * (0.5f / kLog2e), xx = x * x;
+              const float series = __builtin_fmaf(xx, __builtin_fmaf(xx, __builtin_fmaf(xx, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f) * x;
+              const float whole = __builtin_fmaf(2.f, __builtin_amdgcn_rcpf(-1.0f - fast_exp2(a)), 1.f);
+              s[rb][e >> 2][e & 3] = fabsf(x) < 0.25f ? series : whole;
+            }
+        }
+      }
+      if (softcap && !capped) {
         // cap * tanh(x) = cap - 2 cap / (exp(2x) + 1): s becomes -1 / (exp(2x) + 1)
 #pragma unroll
         for (int rb = 0; rb < NRB; rb++)
@@ -540,8 +560,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       }
 #pragma unroll
       for (int rb = 0; rb < NRB; rb++) {
-        slope[rb] = softcap ? 2.f * p.cap_log2e : q_scale[rb];
-        offset[rb] = softcap ? p.cap_log2e : 0.f;
+        slope[rb] = capped ? p.cap_log2e : softcap ? 2.f * p.cap_log2e : q_scale[rb];
+        offset[rb] = softcap && !capped ? p.cap_log2e : 0.f;
         if constexpr (MASKED) {
 #pragma unroll
           for (int h = 0; h < NB / 2; h++) seen_bits[rb][h] = 0;
@@ -598,12 +618,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
         uint32_t bad = 0;  // tokens (bits) whose block is NaN
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const uint32_t expo = v_scale(2 * h + (j >> 2), j & 3);
-          vsc[j] = __uint_as_float(expo);
+          const uint32_t word = v_scale(2 * h + (j >> 2), j & 3);
+          vsc[j] = __uint_as_float(word);
           if constexpr (MASKED) {
             // a NaN block stays out of the product, where a weight of zero would not keep it from the rows that do not see it
-            bad |= expo == 0x7f800000u ? 1u << j : 0u;
-            vsc[j] = expo == 0x7f800000u ? 0.f : vsc[j];
+            const bool is_nan = (word & 0x7f800000u) == 0x7f800000u;
+            bad |= is_nan ? 1u << j : 0u;
+            vsc[j] = is_nan ? 0.f : vsc[j];
           }
         }
         value_operands(
@@ -648,7 +669,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
       __builtin_amdgcn_sched_barrier(0);
       rq_step();
     };
-    for (; tok + kTile <= limit_min && tok < tok_end; tok += kUnit) step(std::false_type{});
+    if (PT || !large_cap)
+      for (; tok + kTile <= limit_min && tok < tok_end; tok += kUnit) step(std::false_type{});
     for (; tok < tok_end; tok += kUnit) step(std::true_type{});
 
     const int u_next = cur.pre + cur.nu;
@@ -856,7 +878,7 @@ const char* launch_fp4(const Fp4Params& p, hipStream_t s) {
   const int64_t pairs = (int64_t)p.n_parts * p.heads_kv;
   const int64_t grid = 8 * (int64_t)p.row_groups * ((pairs + 7) / 8);
   if (grid > INT_MAX) return "too many workgroups";
-  if (p.page_size % kTile == 0)
+  if (p.page_size % kTile == 0 && p.cap_log2e <= kLargeCap)
     hipLaunchKernelGGL((paged_decode_fp4_kernel<QT, D, NRB, true>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, p);
   else
     hipLaunchKernelGGL((paged_decode_fp4_kernel<QT, D, NRB, false>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, p);

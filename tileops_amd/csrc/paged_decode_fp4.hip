@@ -24,8 +24,8 @@
 //
 // Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
 // sequences of 512 .. 8192 tokens, 304 MB in 48 to 52 us, 5.8 to 6.3 TB/s: memory.  64 query heads, 32 sequences of 1024 .. 16384 tokens with
-// eight query tokens and capped scores: 311 MB in 125 to 140 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
-// 270 vector instructions, 48 of them exponentials and reciprocals at half rate, beside 26 matrix instructions.  One sequence of 300
+// eight query tokens and capped scores: 311 MB in 120 to 135 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
+// 250 vector instructions, 48 of them exponentials and reciprocals at half rate, beside 26 matrix instructions.  One sequence of 300
 // tokens: 7.3 us, the chain of loads length, table entry, tile.
 #include <climits>
 #include <type_traits>

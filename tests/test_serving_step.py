@@ -704,9 +704,9 @@ def test_fp4_decode_scales_and_caps_with_wide_tables(kw):
 def test_fp4_decode_with_a_cap_far_above_the_scores(softcap, width):
     """Scores of some tens under a cap of up to 1e7: a cap formed as cap - 2 cap / (exp(2x) + 1) in 32 bits would be off by 2^-24 of it."""
     require_gfx950()
-    for dim, q_len, dtype in ((128, 1, BF16), (64, 5, FP16)):
-        case = _attend_case(dim, dtype, dim, 8, 2, 16, [200, 37, 129], q_len=q_len, width=width)
-        _check_attend(case, 16, q_len, _attend(case, 16, q_len, dtype, softcap=softcap, sm_scale=0.05), softcap=softcap, sm_scale=0.05)
+    for dim, q_len, dtype, page in ((128, 1, BF16, 16), (64, 5, FP16, 16), (128, 3, BF16, 64), (256, 1, FP16, 32)):
+        case = _attend_case(dim, dtype, dim, 8, 2, page, [200, 37, 129], q_len=q_len, width=width)
+        _check_attend(case, page, q_len, _attend(case, page, q_len, dtype, softcap=softcap, sm_scale=0.05), softcap=softcap, sm_scale=0.05)
 
 
 @pytest.mark.gpu
@@ -1155,3 +1155,20 @@ def test_native_host_calls_in_inference_mode_and_small_outputs_of_one_allocation
     del outs, t
     junk = [torch.full((4096,), 7, dtype=torch.int32, device=DEV) for _ in range(50)]
     assert last.tolist() == [1] and len(junk) == 50
+
+
+@pytest.mark.gpu
+def test_calls_without_rows():
+    """No tokens in a step: bookkeeping answers, nothing is written."""
+    require_gfx950()
+    alloc, release, table, free = AllocOp(2, 2, 16, 6), ReleaseOp(2, 2, 16, 6), _int([[3, 4], [5, 0]]), _int([1, 2, 0, 0, 0, 0])
+    a = {n: t[:0] if n in ("q", "k", "v", "positions", "slot_mapping") else t for n, t in _append_args(FP4, device=DEV).items()}
+    order = [*list(a)[:9], "k_cache", "v_cache", "k_scale", "v_scale"]
+    append, gather = AppendOp(4, 2, 128, 16, cache_dtype=FP4), GatherOp(2, 128, 16)
+    for _ in range(2):  # the registered operators, then the native path
+        slots, positions, lens, refused, left = alloc(_int([20, 7]), table, free, _int([2]), _int([0, 0, 0]), 0)
+        assert slots.numel() == positions.numel() == 0 and lens.tolist() == [20, 7] and refused.tolist() == [False] * 2 and left.tolist() == [2]
+        lens, left = release(torch.zeros(2, dtype=torch.bool, device=DEV), lens, table, free, left)
+        assert lens.tolist() == [20, 7] and left.tolist() == [2] and free.tolist() == [1, 2, 0, 0, 0, 0] and table.tolist() == [[3, 4], [5, 0]]
+        assert append(*[a[n] for n in order]).shape == (0, 4, 128) and not a["k_cache"].any() and not a["v_scale"].any()
+        assert [t.shape for t in gather(a["k_cache"], a["v_cache"], a["k_scale"], a["v_scale"], slots)] == [(0, 2, 128)] * 2

@@ -24,7 +24,7 @@
 //
 // Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
 // sequences of 512 .. 8192 tokens, 304 MB in 48 to 52 us, 5.8 to 6.3 TB/s: memory.  64 query heads, 32 sequences of 1024 .. 16384 tokens with
-// eight query tokens and capped scores: 311 MB in 120 to 135 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
+// eight query tokens and capped scores: 311 MB in 115 to 130 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
 // 250 vector instructions, 48 of them exponentials and reciprocals at half rate, beside 26 matrix instructions.  One sequence of 300
 // tokens: 7.3 us, the chain of loads length, table entry, tile.
 #include <climits>
@@ -211,6 +211,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     }
   }
 
+  // Of the two waves on a SIMD the one that was started first goes first: its workgroup is done after 93 us of 130, and the other goes on alone
+  // with a unit half used.  So the second half of the workgroups go first until three quarters of their range (32 x 1024 .. 16384 tokens
+  // with eight query tokens, whole call: 129 us without, 126 / 124 / 123 / 125 with 4 / 5 / 6 / 7 eighths; calls that wait for memory: 1%).
+  const int first_until = !p.by_sequence && blockIdx.x >= gridDim.x / 2 ? u_begin + (int)((int64_t)(u_end - u_begin) * 3 / 4) : 0;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
   const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f, large_cap = p.cap_log2e > kLargeCap;
   const uint32_t q_sign = p.negate_q ? 0x80808080u : 0u;
@@ -505,6 +509,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     // requested there, so a tile's reads have the rest of the step and the head of the next one to arrive.
     auto step = [&](auto masked_tag) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked_tag)::value;
+      if (cur.pre + (int)((uint32_t)tok / kUnit) < first_until) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
       // (products into the same accumulator are kept NRB * NB products apart: back to back each would wait for the one before)
       f32x4 s[NRB][NB];
 #pragma unroll

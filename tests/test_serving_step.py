@@ -1172,3 +1172,14 @@ def test_calls_without_rows():
         assert lens.tolist() == [20, 7] and left.tolist() == [2] and free.tolist() == [1, 2, 0, 0, 0, 0] and table.tolist() == [[3, 4], [5, 0]]
         assert append(*[a[n] for n in order]).shape == (0, 4, 128) and not a["k_cache"].any() and not a["v_scale"].any()
         assert [t.shape for t in gather(a["k_cache"], a["v_cache"], a["k_scale"], a["v_scale"], slots)] == [(0, 2, 128)] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch, width", [(3, 1), (3, 25000), (70, 4000)])
+def test_fp4_decode_of_empty_sequences_is_zeros(batch, width):
+    """Whatever the table's width: no tokens, no ranges, zeros."""
+    require_gfx950()
+    for dim, q_len, dtype in ((128, 1, BF16), (64, 9, FP16), (256, 2, BF16)):
+        case = _attend_case(dim, dtype, dim, 8, 2, 16, [0] * batch, q_len=q_len, width=width)
+        out = _attend(case, 16, q_len, dtype)
+        assert out.dtype == dtype and not out.any()

@@ -313,6 +313,24 @@ def test_alloc_equals_the_plain_allocator(batch, page, width, decode, spare, pad
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch, page, width, spare, pad", [
+    (64, 16, 20, 0, 0), (64, 32, 40, -40, 1500), (128, 16, 20, 3, 7), (192, 1, 64, 0, 0), (960, 16, 6, -60, 5), (1024, 16, 6, 0, 0), (1024 + 64, 16, 5, 2, 2000),
+    (2048 + 512, 8, 4, -99, 0),
+])
+def test_alloc_of_chunks_for_whole_waves_of_sequences(batch, page, width, spare, pad):
+    """A pass whose sequences fill whole waves: the end of its last sequence lies in a word that no other wave may write."""
+    require_gfx950()
+    rng = random.Random(batch + page + width)
+    cached, news, table, free, pool, total = _alloc_case(rng, batch, page, width, False, spare, pad, empty=0.1)
+    assert total > 1024  # (several workgroups of tokens)
+    op = AllocOp(batch, width, page, pool)
+    want = ref_alloc(cached, news, table, free, page, total)
+    for _ in range(3):
+        outs, t = _run_alloc(op, cached, news, table, free, pool, page, total, False)
+        _same_alloc(outs, t, want)
+
+
+@pytest.mark.gpu
 def test_alloc_refuses_what_does_not_fit_and_serves_the_rest():
     require_gfx950()
     page, width = 16, 4

@@ -108,10 +108,13 @@ __global__ __launch_bounds__(kAllocThreads) void kv_alloc_kernel(
       if (served && need > 0) atomicMax(&s_taken, incl);
     }
     if constexpr (kChunks) {
-      s_cu[t] = q0;
+      // (one writer per word: places behind the pass's sequences are nobody's but the end's, which thread nb - 1 writes)
+      if (t < nb) {
+        s_cu[t] = q0;
+        s_cached[t] = c;
+        s_first[t] = served ? first : -1;
+      }
       if (t == nb - 1) s_cu[nb] = q0 + (int)max(n, (int64_t)0);
-      s_cached[t] = c;
-      s_first[t] = served ? first : -1;
       __syncthreads();
       if (tok < total_q && tok >= s_cu[0] && tok < s_cu[nb]) {
         int lo = 0, hi = nb;  // the last sequence that starts at or before the token (empty ones start where the next does)

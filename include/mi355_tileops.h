@@ -292,8 +292,9 @@ int mi355_prefill_input_facts(const int32_t* cu_seqlens_q, const int32_t* cache_
  *   free_pages     [n_pages] int32, a stack: the free pages are free_pages[0 .. free_count[0]), taken from the end
  *   free_count     [1] int32 (read as if clamped to [0, n_pages])
  * Sequence b, with c = cached[b] and n new tokens, needs ceil((c + n) / page_size) - ceil(c / page_size) pages.  Sequences are
- * served in batch order; one is refused if it would outgrow its row (max_pages * page_size tokens, or 2^31 - 1), if c < 0, or if the
- * pages that it and all earlier sequences (that fit their rows) need are more than there are and it needs any.  Page i of the
+ * served in batch order; one is refused if it would outgrow its row (max_pages * page_size tokens, or 2^31 - 1), if c < 0, if its tokens do
+ * not all lie in the step ([0, total_q)), or if the pages that it and all earlier sequences (that fit their rows and lie in the step) need
+ * are more than there are and it needs any.  Page i of the
  * call, counted in batch order and then by logical page, is free_pages[free - 1 - i].
  *   slots          [total_q] int64: page * page_size + offset of each new token; -1 for tokens of refused sequences and tokens that
  *                  belong to no sequence (a padded step)

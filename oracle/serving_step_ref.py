@@ -20,9 +20,9 @@ def ref_alloc(cached, news, table, free, page_size, total_q):
     refused, the pages left and the new table."""
     table = [list(r) for r in table]
     slots, positions, lengths, refused = [], [], [], []
-    wanted = 0  # pages asked for by the sequences that fit their rows, so far
+    wanted = 0  # pages asked for by the sequences that fit their rows and lie in the step, so far
     for b, (c, n) in enumerate(zip(cached, news)):
-        fits = n > 0 and c >= 0 and c + n <= min(len(table[b]) * page_size, 2 ** 31 - 1)
+        fits = n > 0 and c >= 0 and c + n <= min(len(table[b]) * page_size, 2 ** 31 - 1) and len(slots) + n <= total_q
         need = -(-(c + n) // page_size) - -(-c // page_size) if fits else 0
         served = fits and (need == 0 or wanted + need <= len(free))
         if served:
@@ -41,7 +41,7 @@ def ref_alloc(cached, news, table, free, page_size, total_q):
         if lengths[b] != c:
             taken += -(-lengths[b] // page_size) - -(-c // page_size)
     pad = total_q - len(slots)
-    return slots + [-1] * pad, positions + [-1] * pad, lengths, refused, len(free) - taken, table
+    return (slots + [-1] * pad)[:total_q], (positions + [-1] * pad)[:total_q], lengths, refused, len(free) - taken, table
 
 
 def ref_release(finished, lengths, table, free, page_size):

@@ -355,6 +355,27 @@ def test_alloc_refuses_what_does_not_fit_and_serves_the_rest():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch, page, width, spare, short", [(3, 16, 4, 5, 1), (33, 16, 20, 0, 700), (64, 8, 40, -9, 5000), (1100, 16, 6, 3, 9000), (5, 16, 9, 0, 10 ** 9)])
+def test_alloc_refuses_sequences_whose_tokens_do_not_lie_in_the_step(batch, page, width, spare, short):
+    """A step shorter than its sequences' tokens: what reaches past its end is refused whole, and neither its pages leave the list nor does its
+    row change; offsets below zero likewise."""
+    require_gfx950()
+    rng = random.Random(batch + short)
+    cached, news, table, free, pool, total = _alloc_case(rng, batch, page, width, False, spare, 0, empty=0.1)
+    total = max(0, total - short)
+    op = AllocOp(batch, width, page, pool)
+    outs, t = _run_alloc(op, cached, news, table, free, pool, page, total, False)
+    want = ref_alloc(cached, news, table, free, page, total)
+    assert any(want[3])
+    _same_alloc(outs, t, want)
+    # the first sequence begins before the step
+    op, table = AllocOp(2, 2, 16, 6), _int([[7, 7], [8, 8]])
+    slots, positions, lens, refused, left = op(_int([0, 5]), table, _int([0, 1, 2, 3, 4, 5]), _int([6]), _int([-3, 17, 20]), 20)
+    assert slots.tolist() == [-1] * 17 + [8 * 16 + 5 + i for i in range(3)] and positions.tolist() == [-1] * 17 + [5, 6, 7]
+    assert lens.tolist() == [0, 8] and refused.tolist() == [True, False] and left.tolist() == [6] and table.tolist() == [[7, 7], [8, 8]]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch, page, width, share", [(1, 1, 1, 1.0), (3, 16, 5, 0.0), (5, 24, 70, 0.5), (64, 64, 9, 0.3), (1030, 16, 3, 0.7), (2, 16, 400, 1.0)])
 def test_release_equals_the_plain_stack(batch, page, width, share):
     require_gfx950()

@@ -38,7 +38,7 @@ constexpr int kAllocThreads = 1024;
 
 // With c_b tokens cached and n_b to come, sequence b needs need_b = ceil((c_b + n_b) / page) - ceil(c_b / page) pages.  In batch
 // order, page i of the call is free_pages[free - 1 - i] (the list is a stack); b is served if its tokens fit its table row and
-// need_b is 0 or sum_{a <= b} need_a <= free.  A new page's first token lies in this call, so the thread of that token
+// lie in the step, and need_b is 0 or sum_{a <= b} need_a <= free.  A new page's first token lies in this call, so the thread of that token
 // writes the table entry, and token t's page is either an entry that this call leaves alone or a place in the list: no
 // workgroup waits for another.  Every workgroup sums the needs of the sequences up to its own tokens itself (a few loads: 1024
 // sequences a pass); the first one goes through all of them and writes what there is one of per sequence.
@@ -86,7 +86,8 @@ __global__ __launch_bounds__(kAllocThreads) void kv_alloc_kernel(
       n = kChunks ? (int64_t)cu_q[b + 1] - q0 : 1;
       c = cached[b];
     }
-    const bool fits = n > 0 && c >= 0 && c + n <= row_tokens;
+    // (tokens outside the step have no thread to write their pages' entries: their sequence is refused)
+    const bool fits = n > 0 && c >= 0 && c + n <= row_tokens && (!kChunks || (q0 >= 0 && q0 + n <= total_q));
     const int need = fits ? pages_of(c + (int)n, page_size) - pages_of(c, page_size) : 0;
     int incl = wave_sat_scan(need);
     if (lane == 63) s_wave[wave] = incl;

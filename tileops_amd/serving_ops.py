@@ -123,10 +123,10 @@ class PagedKVCacheAllocFwdOp(_ServingOp):
     total_q=None)``, all ``int32``, returns ``(slot_mapping [total_q] int64, positions [total_q] int32, real_seqlen_kv [batch] int32,
     refused [batch] bool, free_count_out [1] int32)`` and writes the block-table entries of the pages that it takes.
 
-    Sequence ``b`` gets the tokens ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]`` of the packed step (one each without ``cu_seqlens_q``);
-    ``total_q`` is the step's length, which may be padded behind the last sequence.  ``free_pages[:free_count]`` is a stack of free
-    pages.  Sequences are served in batch order; one that would outgrow its row, or for which the pages do not last, is ``refused``: its
-    ``real_seqlen_kv`` stays ``cache_seqlens[b]``, and its tokens -- like padding -- have slot and position -1.  ``free_count`` is not
+    Sequence ``b`` gets the tokens ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]`` of the packed step (one each without ``cu_seqlens_q``, whose
+    entries do not decrease); ``total_q`` is the step's length, which may be padded behind the last sequence.  ``free_pages[:free_count]`` is
+    a stack of free pages.  Sequences are served in batch order; one that would outgrow its row, whose tokens do not all lie below
+    ``total_q``, or for which the pages do not last, is ``refused``: its ``real_seqlen_kv`` stays ``cache_seqlens[b]``, and its tokens -- like padding -- have slot and position -1.  ``free_count`` is not
     written (a repeated call gives the same answer): pass ``free_count_out`` to the next step.  The outputs may share one allocation.
     """
 

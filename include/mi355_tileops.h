@@ -328,7 +328,7 @@ int mi355_kv_release(const uint8_t* finished, const int32_t* seqlens, const int3
  * Query rows go to q_out, rounded once to x_dtype.  Key rows (and value rows as they came) go to slot slots[t] of the cache:
  *   16-bit cache (cache_dtype == x_dtype)  [n_phys_tokens, heads_kv, dim], rounded once
  *   FP8 cache                              the same with k_scale, v_scale [n_phys_tokens, heads_kv] fp32: the format and rounding
- *                                          of mi355_kv_append_fp8()
+ *                                          of mi355_kv_append_fp8(); NaN and infinities reach the scale, so that such a row reads as NaN
  *   4-bit cache                            as above, k_scale, v_scale = the scale bytes
  * Norm and rotation are formed in fp32; keys that become codes in fp64, rounded to fp32 once and then to the code, so that codes do
  * not depend on the order of a sum.  Tokens whose slot is outside the pool are not appended (their query row is still written).

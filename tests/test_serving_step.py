@@ -548,6 +548,67 @@ def test_append_of_values_that_are_not_numbers_and_of_the_largest():
     assert empty.shape == (0, 2, 128)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [FP4, FP8, None], ids=["fp4", "fp8", "16"])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("dtype, dim, rotary, interleaved, norm", [
+    (BF16, 128, 0, False, False), (FP16, 64, 64, False, True), (FP16, 128, 64, True, False), (BF16, 256, 128, False, False), (FP16, 256, 256, True, True),
+], ids=str)
+def test_append_of_rows_that_hold_nan_or_infinities(cache, aligned, dtype, dim, rotary, interleaved, norm):
+    """Every cache keeps them: a NaN or an infinity is what the formula makes of it in the 16-bit cache, and a row (FP8) or block (4-bit) that
+    holds one reads as NaN.  Rows aligned to 16 bytes, and to 4 only."""
+    require_gfx950()
+    heads, heads_kv, tokens, page = 4, 2, 12, 16
+    args = _append_inputs(dtype, dim, heads, heads_kv, tokens, cache, rotary, norm, False, page, 21)
+    args["slot_mapping"] = torch.randperm(2 * page, generator=torch.Generator().manual_seed(1))[:tokens]
+    for n in ("q", "k", "v"):
+        x = args[n]
+        x[0, 0, 5], x[0, 1, dim - 1], x[1, 0, 0] = math.nan, math.inf, -math.inf
+        x[2, 0, 3], x[2, 0, 40], x[3, 1, dim // 2], x[3, 1, 1] = math.nan, math.inf, math.inf, -math.inf
+        x[4, 0, 7] = torch.finfo(dtype).max
+        x[5, 1] = math.nan
+        x[6, 0], x[6, 1] = math.inf, 0.0
+        x[7, 0, 9] = -math.nan
+    dev = _to_dev(args)
+    if not aligned:
+        for n in ("q", "k", "v"):
+            dev[n] = torch.cat([dev[n].new_zeros(2), dev[n].flatten()])[2:].view(dev[n].shape)
+            assert dev[n].data_ptr() % 16 == 4
+    eps = 1e-5
+    out = AppendOp(heads, heads_kv, dim, page, rotary_dim=rotary, eps=eps, interleaved=interleaved, cache_dtype=cache)(**dev).cpu()
+    q, k = (ref_norm_rope(args[n], args[n + "_weight"], args["cos_table"], args["sin_table"], args["positions"], eps, interleaved) for n in ("q", "k"))
+
+    def same16(x, ref):  # the bound of _check_append where the result is finite; the type's own rounding decides what overflows
+        ref16 = ref.to(dtype).double()
+        assert torch.equal(x.isnan(), ref16.isnan()) and torch.equal(x.isinf(), ref16.isinf()) and torch.equal(x[x.isinf()].double(), ref16[ref16.isinf()])
+        ok = ref16.isfinite()
+        row = torch.where(ok, ref, 0.0).abs().amax(-1, keepdim=True)
+        err = torch.where(ok, (x.double() - ref).abs(), 0.0)
+        bound = torch.finfo(dtype).eps / 2 * ref.abs() * 1.001 + 2.0 ** -20 * row + _subnormal(dtype)
+        assert bool((err <= torch.where(ok, bound, 0.0)).all())
+
+    same16(out, q)
+    at = args["slot_mapping"]
+    for n, x in (("k", k), ("v", args["v"].double())):
+        got, scale = dev[n + "_cache"].cpu(), dev[n + "_scale"].cpu() if cache else None
+        bad = ~x.float().isfinite()
+        if cache == FP4:
+            # (values, not codes: beside an infinity the norm leaves zeros, of (a w c + b w s) * 0 here and of a * 0 * w * c + b * 0 * w * s there,
+            # which agree but for the zero's sign)
+            _, scales, values = ref_fp4_quantize(x.float())
+            assert torch.equal(scale[at // page, :, at % page], scales)
+            torch.testing.assert_close(ref_fp4_values(got[at // page, :, at % page], scales), values, rtol=0, atol=0, equal_nan=True)
+            assert torch.equal(scales == 255, bad.unflatten(-1, (-1, 32)).any(-1))
+        elif cache == FP8:
+            codes, scales = ref_fp8_quantize(x.float())
+            torch.testing.assert_close(scale[at], scales, rtol=0, atol=0, equal_nan=True)
+            values = got[at].float() * scale[at][..., None]
+            torch.testing.assert_close(values, codes.float() * scales[..., None], rtol=0, atol=0, equal_nan=True)
+            assert torch.equal(values.isnan(), bad.any(-1, keepdim=True).expand_as(values))
+        else:
+            same16(got[at], x)
+
+
 # ------------------------------------------------------------------------------------------------------ rows of the cache
 @pytest.mark.gpu
 @pytest.mark.parametrize("cache", [FP4, FP8, None], ids=["fp4", "fp8", "16"])

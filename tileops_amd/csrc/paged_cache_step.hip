@@ -212,6 +212,12 @@ __device__ __forceinline__ uint32_t fp4_pack(const float* x, uint32_t scale_byte
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// FP8 rows: scale = max(amax, 1e-4) / 448 from the largest magnitude's bit pattern, in whose order NaN and infinities come out on top: the
+// scale says what the row holds.
+__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) { return __uint_as_float(max(amax_bits, __float_as_uint(1e-4f))) / 448.0f; }
+// v / scale as it is encoded.  (The clamp would make a number of a NaN; without a finite scale every quotient is NaN or zero.)
+__device__ __forceinline__ float fp8_clamp(float z, float scale) { return scale < __builtin_inff() ? fminf(fmaxf(z, -448.0f), 448.0f) : z; }
+
 // ------------------------------------------------------------------------------- norm + rotation + append of new rows
 struct AppendParams {
   const uint16_t *q, *k, *v;
@@ -328,20 +334,20 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(const AppendPa
     return;
   }
   if (CACHE == kCacheFp8) {
-    float amax = 0.f;
+    uint32_t amax = 0;
 #pragma unroll
     for (int j = 0; j < 2; j++)
-      if (lane + 64 * j < pairs) amax = fmaxf(amax, fmaxf(fabsf(y[j][0]), fabsf(y[j][1])));
+      if (lane + 64 * j < pairs) amax = max(amax, max(abs_bits(y[j][0]), abs_bits(y[j][1])));
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
-    const float sc = fmaxf(amax, 1e-4f) / 448.0f;
+    for (int m = 1; m < 64; m <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, m, 64));
+    const float sc = fp8_scale(amax);
     if (lane == 0) ((float*)(is_k ? p.k_scale : p.v_scale))[token_row] = sc;
     uint8_t* dst = (uint8_t*)(is_k ? p.k_cache : p.v_cache) + token_row * p.dim;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int i = lane + 64 * j;
       if (i >= pairs) continue;
-      const float a = fminf(fmaxf(y[j][0] / sc, -448.0f), 448.0f), b = fminf(fmaxf(y[j][1] / sc, -448.0f), 448.0f);
+      const float a = fp8_clamp(y[j][0] / sc, sc), b = fp8_clamp(y[j][1] / sc, sc);
       ((uint16_t*)dst)[i] = (uint16_t)(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0u, false) & 0xffff);
     }
     return;
@@ -494,13 +500,13 @@ __device__ __forceinline__ void store_cached(const AppendParams& p, void* cache,
   if constexpr (CACHE == kCache16) {
     if (store) *(u32x4*)((uint16_t*)cache + token_row * p.dim + 8 * j) = pack_row8<XT>(y);
   } else if constexpr (CACHE == kCacheFp8) {
-    float amax = 0.f;
+    uint32_t amax = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(y[e]));
-    amax = over_row(amax, lanes, [](float a, float b) { return fmaxf(a, b); });
-    const float sc = fmaxf(amax, 1e-4f) / 448.0f;
+    for (int e = 0; e < 8; e++) amax = max(amax, abs_bits(y[e]));
+    amax = over_row(amax, lanes, [](uint32_t a, uint32_t b) { return max(a, b); });
+    const float sc = fp8_scale(amax);
     const Quotient over(sc);
-    const bool plain = sc < 0x1p100f;  // (else an infinity or close to one: the division itself)
+    const bool plain = sc < 0x1p100f;  // (else NaN, an infinity or close to one: the division itself)
     u32x2 o;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -508,7 +514,7 @@ __device__ __forceinline__ void store_cached(const AppendParams& p, void* cache,
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const float v = y[4 * e + k];
-        z[k] = fminf(fmaxf(plain ? over(v) : v / sc, -448.0f), 448.0f);
+        z[k] = fp8_clamp(plain ? over(v) : v / sc, sc);
       }
       const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
       o[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);

@@ -884,6 +884,35 @@ def test_fp4_decode_rows_do_not_see_what_is_masked(width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, dim, heads, heads_kv, page, q_len", [
+    (BF16, 128, 4, 1, 16, 8), (FP16, 128, 8, 2, 64, 1), (BF16, 64, 6, 2, 16, 17), (FP16, 64, 2, 2, 48, 3), (BF16, 256, 4, 2, 32, 5), (FP16, 256, 2, 1, 16, 2),
+], ids=str)
+@pytest.mark.parametrize("width", [None, 25000])
+def test_fp4_decode_rows_do_not_see_infinities_that_are_masked(dtype, dim, heads, heads_kv, page, q_len, width):
+    """Scale bytes 253 and 254 make 2^128 and more of the larger codes, which no 32-bit number is: in places behind a sequence's end, and in
+    tokens that only later queries see, they leave every row that does not see them as it is, bit for bit."""
+    require_gfx950()
+    lens = [200, q_len, 31, 128, 129]
+    case = _attend_case(dim + q_len, dtype, dim, heads, heads_kv, page, lens, q_len=q_len, width=width)
+    q, k, v, ks, vs, _, table = case
+    clean = (q, k, v, *(torch.where(s == 255, 127, s).to(torch.uint8) for s in (ks, vs)), *case[5:])
+    want = _attend(clean, page, q_len, dtype)
+    g = torch.Generator().manual_seed(dim)
+    filled = [torch.where(s == 255, torch.randint(253, 255, s.shape, generator=g), s).to(torch.uint8) for s in (ks, vs)]
+    assert torch.equal(_attend((q, k, v, *filled, *case[5:]), page, q_len, dtype), want)
+    if q_len > 1:
+        sees = torch.zeros(want.shape, dtype=torch.bool)
+        for b, n in enumerate(lens):
+            if n < q_len:
+                continue
+            token, h, block, first = n - 1, heads_kv - 1, dim // 32 - 1, q_len - 1  # the last token, seen by the last query alone
+            filled[1][table[b, token // page].long(), h, token % page, block] = 253 + b % 2
+            sees[b, first:, h * (heads // heads_kv):, 32 * block:] = True
+        out = _attend((q, k, v, *filled, *case[5:]), page, q_len, dtype)
+        assert torch.equal(out[~sees], want[~sees])
+
+
+@pytest.mark.gpu
 def test_fp4_decode_clamps_lengths_and_page_ids():
     require_gfx950()
     case = _attend_case(4, BF16, 128, 4, 1, 16, [64, 48, 20], width=4)

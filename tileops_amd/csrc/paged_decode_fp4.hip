@@ -621,7 +621,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
 #pragma unroll
       for (int h = 0; h < NB / 2; h++) {
         float vsc[8];
-        uint32_t bad = 0;  // tokens (bits) whose block is NaN
+        uint32_t bad = 0;       // tokens (bits) whose block is NaN
+        bool infinite = false;  // a block's larger codes are infinities (2^128 and more: scale bytes 253 and 254)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const uint32_t word = v_scale(2 * h + (j >> 2), j & 3);
@@ -630,7 +631,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
             // a NaN block stays out of the product, where a weight of zero would not keep it from the rows that do not see it
             const bool is_nan = (word & 0x7f800000u) == 0x7f800000u;
             bad |= is_nan ? 1u << j : 0u;
+            infinite |= !is_nan && (word & 0x7f800000u) >= 253u << 23;
             vsc[j] = is_nan ? 0.f : vsc[j];
+          }
+        }
+        // Infinities would reach them likewise: such a tile enters at a sixteenth, as the numbers that its codes are.  (A scale below 2^-123 stays
+        // what it is or loses less than a sixteenth leaves of it: 2^-120 beside values of 2^126.)
+        bool sixteenth = false;
+        if constexpr (MASKED) {
+          sixteenth = __ballot(infinite) != 0;
+          if (sixteenth) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const uint32_t word = __float_as_uint(vsc[j]);
+              vsc[j] = __uint_as_float(word - min(word & 0x7f800000u, 4u << 23));
+            }
+#pragma unroll
+            for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+              for (int n = 0; n < DPL; n++) o[rb][n] *= 0.0625f;
           }
         }
         value_operands(
@@ -651,6 +670,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
                   o[rb][n] = mma_bf16(a, u32x4{pw[rb][h][q][0], pw[rb][h][q][1], pw[rb][h][q][2], pw[rb][h][q][3]}, o[rb][n]);
             });
         if constexpr (MASKED) {
+          if (sixteenth) {
+#pragma unroll
+            for (int rb = 0; rb < NRB; rb++)
+#pragma unroll
+              for (int n = 0; n < DPL; n++) o[rb][n] *= 16.f;
+          }
           if (__ballot(bad != 0u)) {
             // rows that see a token with a NaN block get NaN there: count such tokens with the same product, 1 for every
             // NaN block against 1 for every visible token

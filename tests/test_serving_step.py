@@ -7,6 +7,7 @@ kernels make; each test states them where it forms them.  Refusals need no GPU.
 import itertools
 import math
 import random
+import warnings
 
 import pytest
 import torch
@@ -1244,6 +1245,38 @@ def test_calls_that_the_native_host_path_leaves_to_python(monkeypatch):
         op(*args)
         assert calls.taken[-1][1], name
         monkeypatch.setattr(native, "_hostcall", calls.module)
+
+
+@pytest.mark.gpu
+def test_a_traced_call_is_recorded_as_its_operator(monkeypatch):
+    """torch.jit.trace of an op that has served calls before: one node of its operator, which computes -- and writes -- anew on every run."""
+    require_gfx950()
+    native.hostcall()
+    for op, args, written in _host_cases():
+        op(*[_clone(x) for x in args])
+        name, at = type(op).__name__, [i for i, x in enumerate(args) if isinstance(x, torch.Tensor)]
+
+        def call(*tensors):
+            given = dict(zip(at, tensors))
+            return op(*(given.get(i, x) for i, x in enumerate(args)))
+
+        calls = _Calls(native.hostcall())
+        monkeypatch.setattr(native, "_hostcall", calls)
+        with warnings.catch_warnings():
+            warnings.simplefilter("ignore")  # (the checks compare shapes, which a trace takes as constants)
+            traced = torch.jit.trace(call, tuple(_clone(args[i]) for i in at), check_trace=False)
+        assert not any(ok for _, ok in calls.taken), name
+        monkeypatch.setattr(native, "_hostcall", calls.module)
+        assert [n.kind() for n in traced.graph.nodes() if n.kind().startswith("tileops_amd::")] == list(op.compile_op_names), (name, traced.graph)
+        for _ in range(2):  # other inputs than the trace's: what is written or read in place, and rows, as they are after a call
+            mine, theirs = ([_clone(x) for x in args] for _ in range(2))
+            for x in (mine, theirs):
+                for i, t in enumerate(x):
+                    if isinstance(t, torch.Tensor) and t.dtype in (BF16, torch.uint8) and i not in written:
+                        t.copy_(t.flip(0))
+            want, got = op(*mine), traced(*(theirs[i] for i in at))
+            assert all(torch.equal(a, b) for a, b in zip(_bytes(want), _bytes(got), strict=True)), name
+            assert all(torch.equal(a, b) for a, b in zip(_bytes(tuple(mine)), _bytes(tuple(theirs)), strict=True)), name
 
 
 @pytest.mark.gpu

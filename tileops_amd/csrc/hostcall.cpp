@@ -5,8 +5,8 @@
 // 64 sequences 16.8 / 5.9 us (7.5 with an allocation per output), release 12.8 / 5.5 us, append + rows read back 36.8 / 12 us, attention over
 // 300 tokens 17.8 / 6.3 us (less than its kernel takes).
 //
-// Every function here returns None when a call is not for it -- a tensor that is not a plain one on the current device, a gradient or a
-// dispatch mode in force, a check that does not hold -- and has then done nothing: the op's Python path takes the call and says what
+// Every function here returns None when a call is not for it -- a tensor that is not a plain one on the current device, a gradient, a
+// tracer or a dispatch mode in force, a check that does not hold -- and has then done nothing: the op's Python path takes the call and says what
 // is wrong with it.  Otherwise it returns the outputs, or the C entry point's negative error code.
 #include <Python.h>
 
@@ -33,7 +33,8 @@ using at::Tensor;
 const c10::DispatchKeySet kNotPlain({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
                                      c10::DispatchKey::ZeroTensor, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
                                      c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Batched,
-                                     c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode});
+                                     c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
+                                     c10::DispatchKey::Tracer});
 
 // The conditions of one call: a device index that is the current one, and no mode that wants to see the call.
 struct Call {

@@ -1248,6 +1248,41 @@ def test_calls_that_the_native_host_path_leaves_to_python(monkeypatch):
 
 
 @pytest.mark.gpu
+def test_function_modes_see_the_operators_and_a_default_device_does_not_count(monkeypatch):
+    from torch.overrides import TorchFunctionMode
+
+    require_gfx950()
+    native.hostcall()
+
+    class Names(TorchFunctionMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for op, args, _ in _host_cases():
+        want, name = op(*[_clone(x) for x in args]), type(op).__name__
+        calls = _Calls(native.hostcall())
+        monkeypatch.setattr(native, "_hostcall", calls)
+        with Names() as mode:
+            got = op(*args)
+        assert not any(ok for _, ok in calls.taken), name
+        assert any(op.compile_op_names[0].replace("::", ".") in n for n in mode.names), (name, mode.names)
+        with torch.device(DEV):
+            with Names():
+                op(*args)
+            assert not any(ok for _, ok in calls.taken), name
+            again = op(*args)
+        assert calls.taken[-1][1], name
+        monkeypatch.setattr(native, "_hostcall", calls.module)
+        for out in (got, again):
+            assert all(torch.equal(a, b) for a, b in zip(_bytes(want), _bytes(out), strict=True)), name
+
+
+@pytest.mark.gpu
 def test_a_traced_call_is_recorded_as_its_operator(monkeypatch):
     """torch.jit.trace of an op that has served calls before: one node of its operator, which computes -- and writes -- anew on every run."""
     require_gfx950()

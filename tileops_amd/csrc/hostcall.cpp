@@ -6,17 +6,19 @@
 // 300 tokens 17.8 / 6.3 us (less than its kernel takes).
 //
 // Every function here returns None when a call is not for it -- a tensor that is not a plain one on the current device, a gradient, a
-// tracer or a dispatch mode in force, a check that does not hold -- and has then done nothing: the op's Python path takes the call and says what
+// tracer, a dispatch mode or a function mode in force, a check that does not hold -- and has then done nothing: the op's Python path takes the call and says what
 // is wrong with it.  Otherwise it returns the outputs, or the C entry point's negative error code.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -36,12 +38,23 @@ const c10::DispatchKeySet kNotPlain({c10::DispatchKey::Python, c10::DispatchKey:
                                      c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
                                      c10::DispatchKey::Tracer});
 
+// Modes on the level of torch's functions want to see the call, all but the one that a default device sets: it only fills in the device
+// of factory functions, and programs keep it set.
+PyTypeObject* g_default_device_mode = nullptr;
+bool function_modes() {
+  using Stack = at::impl::PythonTorchFunctionTLS;
+  if (!at::impl::torch_function_mode_enabled()) return false;
+  for (int64_t i = 0; i < Stack::stack_len(); i++)
+    if (Py_TYPE(Stack::get_stack_at(i)->ptr(getPyInterpreter())) != g_default_device_mode) return true;
+  return false;
+}
+
 // The conditions of one call: a device index that is the current one, and no mode that wants to see the call.
 struct Call {
   c10::Device device;
   bool ok, grad;
   explicit Call(long index) : device(c10::DeviceType::CUDA, (c10::DeviceIndex)index), grad(at::GradMode::is_enabled()) {
-    ok = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !c10::impl::tls_local_dispatch_key_set().included_.has_any(kNotPlain) &&
+    ok = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !function_modes() && !c10::impl::tls_local_dispatch_key_set().included_.has_any(kNotPlain) &&
          c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice() == device;
   }
   const Tensor* plain(PyObject* o) {
@@ -345,4 +358,10 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_hostcall", nullptr, -1, kMethods
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__hostcall(void) { return PyModule_Create(&kModule); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__hostcall(void) {
+  PyObject* device = PyImport_ImportModule("torch.utils._device");
+  if (!device) return nullptr;
+  g_default_device_mode = (PyTypeObject*)PyObject_GetAttrString(device, "DeviceContext");  // (kept for the life of the process)
+  Py_DECREF(device);
+  return g_default_device_mode ? PyModule_Create(&kModule) : nullptr;
+}

@@ -69,7 +69,7 @@ class _ServingOp(Op):
     """What the ops of this module share: one kernel class per op, and the native host path.
 
     A call goes the long way -- the checks below, kernel selection, the registered operator -- the first time, on any other device than
-    that one, under a tracer or a dispatch mode, with gradients or an external target, and whenever something is wrong with it.  Otherwise
+    that one, under a tracer, a dispatch mode or a function mode, with gradients or an external target, and whenever something is wrong with it.  Otherwise
     ``hostcall`` (csrc/hostcall.cpp) does the same checks and the launch in one native call, or answers None: then the long way is taken.
     """
 

@@ -811,6 +811,37 @@ def test_fp4_decode_with_a_cap_far_above_the_scores(softcap, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("dim, heads, heads_kv, q_len, page", [(128, 4, 2, 1, 16), (64, 3, 1, 6, 64), (256, 4, 2, 2, 16), (128, 40, 1, 1, 32)])
+@pytest.mark.parametrize("equal", [True, False])
+def test_fp4_decode_of_small_query_elements_beside_a_large_one(dtype, dim, heads, heads_kv, q_len, page, equal):
+    """A channel with a large query meets keys of zero, the others, 2^-9 to 2^-16 of it, decide the scores.  The query's e4m3 rows reach down to
+    2^-22 (fp16: 2^-27) of the row's largest element, which moves a logit by dz at most; all other roundings as in _check_attend."""
+    require_gfx950()
+    lens = [150, 31]
+    q, k, v, ks, vs, lens_t, table = _attend_case(dim + heads, dtype, dim, heads, heads_kv, page, lens, q_len=q_len)
+    g = torch.Generator().manual_seed(dim)
+    # keys: one magnitude for all channels of a token, which tells the tokens apart; channel 0 is zero
+    index = torch.randint(0, 8, (*k.shape[:3], 1), generator=g)
+    k = (index * 17).expand(k.shape).to(torch.uint8).contiguous()
+    k[..., 0] &= 0xf0
+    ks = torch.where(ks == 255, 255, 139).to(torch.uint8) if equal else torch.where(ks == 255, 255, 138).to(torch.uint8)
+    q = torch.full(q.shape, 191 / 128 * 2.0 ** -16)
+    if not equal:
+        q = q * torch.exp2(6 * torch.rand(q.shape, generator=g)) * torch.where(torch.rand(q.shape, generator=g) < 0.3, -1.0, 1.0)
+    q[..., 0] = 1.0
+    q = q.to(dtype)
+    case = (q, k, v, ks, vs, lens_t, table)
+    out = _attend(case, page, q_len, dtype)
+    ref, spread, reach = ref_attention(q, ref_fp4_values(k, ks), ref_fp4_values(v, vs), lens_t, table, page, sm_scale=dim ** -0.5)
+    dz = (2.0 ** -22 if dtype == BF16 else 2.0 ** -27) * reach * dim ** -0.5
+    assert dz.max() < 0.6  # (the channels' scores are some times larger)
+    bound = torch.finfo(dtype).eps / 2 * ref.abs() * 1.01 + ((2.0 ** -8 if dtype == BF16 else 2.0 ** -16) + 2 * dz + 2.0 ** -13) * spread + _subnormal(dtype)
+    off = (out.double() - ref).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, dim, heads, heads_kv, q_len", [(BF16, 128, 8, 1, 1), (FP16, 64, 2, 1, 1), (BF16, 256, 4, 4, 1), (BF16, 128, 16, 2, 4)])
 def test_fp4_decode_joins_many_ranges(dtype, dim, heads, heads_kv, q_len):
     """Few sequences in many ranges, so that a workgroup joins a row's; one that lies in a single range and one without tokens beside it."""

@@ -11,15 +11,15 @@
 //    the others leave normalised fp32 rows with log-sum-exps for the merge kernel.  Where the block tables address few tokens
 //    a range is a sequence: nothing is left to merge.
 //  * Q.K^T: v_mfma_scale_f32_16x16x128_f8f6f4 with the K codes as they lie in memory -- lane (c, g) supplies block g of token
-//    c, sixteen bytes, and its scale byte -- against the query row as a sum of two (bf16: exact) or three (fp16: exact) e4m3 rows.
+//    c, sixteen bytes, and its scale byte -- against the query row as a sum of two (bf16) or three (fp16) e4m3 rows with scales of their own.
 //    Tokens sit on the M axis, so every softmax quantity of a query row is local to a lane column.
 //  * PV: O^T += V^T.P^T on v_mfma_f32_16x16x32_bf16.  Lane (c, g) loads the head elements [c * D/16, (c + 1) * D/16) of its eight
 //    tokens -- those whose probabilities it holds already -- widens them with their scale (v_cvt_scalef32_pk_bf16_fp4) and pairs the
 //    tokens with byte permutes: V needs no LDS, P does not move.
 //  * K, V and scales go from memory to registers, a tile ahead of their use, across the borders of sequences.
 //
-// Roundings: the query's e4m3 rows add up to it exactly (fp16 elements far below their row's largest excepted: 2^-17 of that one); a
-// probability becomes one bf16 (two for fp16 queries, whose rows carry three bits more), because PV then runs at the rate of 16-bit
+// Roundings: the query's e4m3 rows add up to its elements down to 2^-14 (fp16: 2^-16) of the row's largest, smaller ones are off by 2^-22 (2^-27)
+// of that one at most; a probability becomes one bf16 (two for fp16 queries, whose rows carry three bits more), because PV then runs at the rate of 16-bit
 // products, and the row's sum is formed of the rounded ones, so that a common error cancels.  All else is fp32.
 //
 // Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
@@ -115,6 +115,13 @@ __device__ __forceinline__ f32x4 mma_bf16(u32x4 a, u32x4 b, f32x4 c) {
 }
 template <int SEL> __device__ __forceinline__ uint32_t widen2(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+}
+
+// Sixteen tokens' K codes against sixteen query rows; SEL: byte of b_scales that is the scale byte of the lane's block of the query operand.
+template <int SEL> __device__ __forceinline__ f32x4 mma_codes(u32x4 k, u32x4 b0, u32x4 b1, f32x4 c, uint32_t k_scale, uint32_t b_scales) {
+  const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, (int)k_scale, SEL, (int)b_scales);
 }
 
 // (a constant-address-space load of a wave-uniform address is a scalar load: the block table does not pass through the
@@ -221,6 +228,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   // byte of the lane's block in a word of V scales (head dim 64: of the first of the word's two tokens), turned right by this
   // many bits, sits in a float's exponent
   const uint32_t v_turn = (8 * (D == 64 ? c >> 3 : D == 128 ? c >> 2 : (c >> 1) & 3) + 9) & 31;
+  // scale bytes of the query operands, one for each row n of its taking apart: 2^(-5n) (head dim 64: two rows side by side, in blocks 0, 1 and 2, 3)
+  const uint32_t q_bytes = D == 64 ? (g < 2 ? 0x757fu : 0x707au) : 0x757a7fu;
   // what the lane reads of a block of sixteen tokens: K row c, block g (head dim 64: g % 2); V rows 4g .. 4g + 3, elements c * DPL ..
   const uint32_t k_lane = c * ROW + 16 * (D == 64 ? g & 1 : g), ks_lane = (D == 64 ? c & ~1 : c) * (ROW / 16);
   const uint32_t k_shift = D == 64 ? 16 * (c & 1) + 8 * (g & 1) : 8 * g;  // of the lane's scale byte in the word it reads
@@ -408,7 +417,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
     const bool whole = cur.u0 == 0 && cur.u1 == cur.nu;
     int tok = cur.tok;
 
-    // query rows: scaled by a power of two that puts the row's largest magnitude in [128, 256), then taken apart into e4m3 rows
+    // query rows: scaled by a power of two that puts the row's largest magnitude in [128, 256), then taken apart into e4m3 rows, each 32 times
+    // the remainder of the one before (8 at most; the operand's scale byte takes the factor back), so that small elements lose nothing
     u32x4 qf[NRB][KD][NQM][2];
     float q_scale[NRB];
     int limit[NRB];
@@ -445,10 +455,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
           for (int n = 0; n < NQ; n++) {
             const uint32_t word = pack_fp8x4(a[0], a[1], a[2], a[3]);
             const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-            a[0] -= lo[0];
-            a[1] -= lo[1];
-            a[2] -= hi[0];
-            a[3] -= hi[1];
+            a[0] = (a[0] - lo[0]) * 32.f;
+            a[1] = (a[1] - lo[1]) * 32.f;
+            a[2] = (a[2] - hi[0]) * 32.f;
+            a[3] = (a[3] - hi[1]) * 32.f;
             parts[h][n][w] = word ^ q_sign;
           }
         }
@@ -521,11 +531,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
           for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int rb = 0; rb < NRB; rb++) {
-              const u32x4 kk = kr[i][kd], b0 = qf[rb][kd][n][0], b1 = qf[rb][kd][n][1];
-              const i32x8 a = {(int)kk[0], (int)kk[1], (int)kk[2], (int)kk[3], 0, 0, 0, 0};
-              const i32x8 bq = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
               const f32x4 sum = kd + n == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rb][i];
-              s[rb][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bq, sum, 4, 0, 0, (int)(ksr[i][kd] >> k_shift), 0, 127);
+              const u32x4 b0 = qf[rb][kd][n][0], b1 = qf[rb][kd][n][1];
+              const uint32_t k_byte = ksr[i][kd] >> k_shift;
+              s[rb][i] = n == 0 ? mma_codes<0>(kr[i][kd], b0, b1, sum, k_byte, q_bytes)
+                         : n == 1 ? mma_codes<1>(kr[i][kd], b0, b1, sum, k_byte, q_bytes) : mma_codes<2>(kr[i][kd], b0, b1, sum, k_byte, q_bytes);
             }
           __builtin_amdgcn_sched_barrier(0);
         }

@@ -362,7 +362,8 @@ int mi355_kv_gather_fp4(const void* k_codes, const void* v_codes, const void* k_
  * A query row that sees no token (seqlens[b] == 0, or causal with q_len > seqlens[b]) is zeros.  Tokens that a row does not see
  * do not change it, whatever their bytes are.  Values of 2^128 and more (scale bytes 253 and 254) may enter the rows that see them as
  * infinities.  Both products accumulate in fp32; the query enters exactly (up to 2^-22, fp16 2^-27, of the
- * row's largest element), probabilities as bf16 (fp16 queries: as two bf16 parts).
+ * row's largest element), probabilities as two bf16 parts (as one, in calls of more than sixteen rows per kv head
+ * -- q_len * heads / heads_kv -- with bf16 queries and head dim 64 or 128).
  * The query of the workspace's size touches no device; partial results are fp32.
  */
 int mi355_gqa_paged_decode_fp4_workspace(int batch, int q_len, int heads, int heads_kv, int dim, int page_size, int q_dtype,

@@ -736,7 +736,7 @@ def _attend(case, page, q_len, dtype, **kw):
     return out.reshape(q.shape).cpu()
 
 
-def _check_attend(case, page, q_len, out, sm_scale=None, softcap=0.0, causal=True):
+def _check_attend(case, page, q_len, out, sm_scale=None, softcap=0.0, causal=True, parts=None):
     """Bound on an element's error: the output's rounding (half a step of its type), each probability's rounding to bf16 (2^-8; two
     parts with fp16 queries: 2^-16), the query's e4m3 parts (2^-17 of its largest element, times the sum of |k|, moves a logit by
     dz and a normalised probability by a factor of 2 dz at most) and 2^-13 for the logits' and sums' own 32-bit roundings.
@@ -748,8 +748,9 @@ def _check_attend(case, page, q_len, out, sm_scale=None, softcap=0.0, causal=Tru
     sm_scale = D ** -0.5 if sm_scale is None else sm_scale
     ref, spread, reach = ref_attention(q, ref_fp4_values(k, ks), ref_fp4_values(v, vs), lens, table, page, sm_scale=sm_scale, softcap=softcap, causal=causal)
     half_step = torch.finfo(q.dtype).eps / 2
+    parts = parts or (1 if q.dtype == BF16 else 2)
     dz = 2.0 ** -17 * q.double().abs().amax(-1, keepdim=True) * reach * abs(sm_scale)
-    bound = half_step * ref.abs() * 1.01 + ((2.0 ** -8 if q.dtype == BF16 else 2.0 ** -16) + 2 * dz + 2.0 ** -13) * spread + _subnormal(q.dtype)
+    bound = half_step * ref.abs() * 1.01 + (2.0 ** (-8 * parts) + 2 * dz + 2.0 ** -13) * spread + _subnormal(q.dtype)
     largest = ref_fp4_values(v, vs).double().abs().nan_to_num(nan=1.0).max().clamp(min=1)
     bound = bound + 2.0 ** -124 * lens.double().reshape(-1, 1, 1, 1) * largest
     off = (out.double() - ref).abs()
@@ -808,6 +809,17 @@ def test_fp4_decode_with_a_cap_far_above_the_scores(softcap, width):
     for dim, q_len, dtype, page in ((128, 1, BF16, 16), (64, 5, FP16, 16), (128, 3, BF16, 64), (256, 1, FP16, 32)):
         case = _attend_case(dim, dtype, dim, 8, 2, page, [200, 37, 129], q_len=q_len, width=width)
         _check_attend(case, page, q_len, _attend(case, page, q_len, dtype, softcap=softcap, sm_scale=0.05), softcap=softcap, sm_scale=0.05)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim, heads, heads_kv, q_len, page", [(128, 32, 2, 1, 16), (64, 6, 1, 2, 64), (256, 24, 1, 1, 16), (128, 8, 4, 5, 32), (64, 16, 1, 1, 48)])
+@pytest.mark.parametrize("width", [None, 25000])
+def test_fp4_decode_holds_probabilities_in_two_parts(dim, heads, heads_kv, q_len, page, width):
+    """Calls of at most sixteen rows per kv head (any number at head dim 256): bf16 queries, too, with 2^-16 of a probability instead of 2^-8.  Few tokens, whose
+    rounding errors do not average out."""
+    require_gfx950()
+    case = _attend_case(dim + heads, BF16, dim, heads, heads_kv, page, [3, 9, 17, 33, 5, 2, 7, 300], q_len=q_len, width=width)
+    _check_attend(case, page, q_len, _attend(case, page, q_len, BF16), parts=2)
 
 
 @pytest.mark.gpu

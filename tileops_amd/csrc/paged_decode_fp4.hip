@@ -19,8 +19,11 @@
 //  * K, V and scales go from memory to registers, a tile ahead of their use, across the borders of sequences.
 //
 // Roundings: the query's e4m3 rows add up to its elements down to 2^-14 (fp16: 2^-16) of the row's largest, smaller ones are off by 2^-22 (2^-27)
-// of that one at most; a probability becomes one bf16 (two for fp16 queries, whose rows carry three bits more), because PV then runs at the rate of 16-bit
-// products, and the row's sum is formed of the rounded ones, so that a common error cancels.  All else is fp32.
+// of that one at most; a probability becomes two bf16 (2^-17 of it), because PV then runs at the rate of 16-bit products.  Waves with two blocks of
+// rows and bf16 queries make do with one bf16 (2^-9; the output's own rounding is that large): they are bound by the vector unit, where
+// the second part takes 40 instructions and 18 products a tile (32 x 1024 .. 16384 tokens with eight query tokens: 115 to 123 us, with both 142 to 154; calls with
+// one block: 8 x 131072 tokens 180 / 183 us, 64 ragged 56 / 55, 1 x 300 7.3 / 7.3).  The row's sum is formed of the rounded ones, so that a
+// common error cancels.  All else is fp32.
 //
 // Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
 // sequences of 512 .. 8192 tokens, 304 MB in 48 to 52 us, 5.8 to 6.3 TB/s: memory.  64 query heads, 32 sequences of 1024 .. 16384 tokens with
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   constexpr int KD = D <= 128 ? 1 : 2;          // 128-deep steps of Q.K^T = 32-element blocks of a K row per lane
   constexpr int NQ = F16 ? 3 : 2;               // e4m3 rows that add up to the query row
   constexpr int NQM = D == 64 ? (NQ + 1) / 2 : NQ;  // matrix operands of them (head dim 64: two rows side by side in the depth)
-  constexpr int NP = F16 ? 2 : 1;               // bf16 parts of a probability
+  constexpr int NP = F16 || NRB == 1 ? 2 : 1;   // bf16 parts of a probability (see above)
   constexpr int DPL = D / 16;                   // head elements per lane of the PV operand
   constexpr int VW = D <= 128 ? 1 : 2;          // dwords of them per token (head dim 64: half a dword)
   constexpr int NB = kTile / 16;                // blocks of sixteen tokens in a tile

@@ -6,6 +6,7 @@ kernels make; each test states them where it forms them.  Refusals need no GPU.
 
 import itertools
 import math
+import pickle
 import random
 import warnings
 
@@ -249,6 +250,22 @@ def test_entry_points_check_their_arguments_and_the_device():
     with pytest.raises(NotImplementedError, match="multiple of 16"):
         native.decode_fp4_workspace(2, 1, 4, 2, 128, 24, BF16)
     assert tileops_amd.__version__
+
+
+def test_an_op_from_another_process_does_not_need_its_host_module(monkeypatch):
+    """An instance that has served a call, pickled and loaded where the host module is not: it checks and speaks like a new one."""
+    a = _append_args(FP4)
+    for op, args in ((AllocOp(2, 4, 16, 9), _alloc_args()), (ReleaseOp(2, 4, 16, 9), [torch.zeros(2, dtype=torch.bool), *_alloc_args()]),
+                     (AppendOp(4, 2, 128, 16, cache_dtype=FP4), [*a.values()]), (GatherOp(2, 128, 16), [*_decode_args().values()][1:6]),
+                     (FP4DecodeOp(2, 4, 2, 64, 128, 16), [*_decode_args().values()])):
+        op._device, op._builder = 0, None
+        if isinstance(op, FP4DecodeOp):
+            op._plans[BF16] = (0, 0)
+        op = pickle.loads(pickle.dumps(op))
+        monkeypatch.setattr(native, "_hostcall", None)
+        with pytest.raises(ValueError, match="must be a torch.Tensor|must be a tensor|must have shape"):
+            op(None, *([None] * (len(args) - 1)))
+        assert not op._native()
 
 
 # ------------------------------------------------------------------------------------------------------- pages on the GPU

@@ -88,7 +88,7 @@ class _ServingOp(Op):
         self.dispatch_kernel(kernel_map)
 
     def _native(self) -> bool:
-        return (self._device is not None and self._builder is None and self.kernel_map[self._key] is self._kernel_class
+        return (self._device is not None and native._hostcall is not None and self._builder is None and self.kernel_map[self._key] is self._kernel_class
                 and not torch.compiler.is_compiling())
 
     @staticmethod
@@ -110,7 +110,8 @@ class _ServingOp(Op):
             kernel = self.get_or_build_kernel(key, inputs, key=(device, dtype, self.kernel_map[key]),
                                               build=lambda: self.kernel_map[key](self, device_index=index))
             self._selected[memo] = kernel
-        if self._device is None and device.type == "cuda" and device.index is not None and not torch.compiler.is_compiling():
+        if ((self._device is None or native._hostcall is None) and device.type == "cuda" and device.index is not None
+                and not torch.compiler.is_compiling()):  # (no module: the instance comes from another process)
             native.hostcall()
             self._device = device.index
         return kernel

@@ -96,6 +96,31 @@ def test_one_manifest_row_end_to_end(tmp_path):
     assert torch.cuda.is_available()
 
 
+def test_every_manifest_workload_has_a_generator():
+    from tileops_amd.manifest import load_manifest
+
+    with_workloads = {name for name, entry in load_manifest().items() if entry.get("workloads")}
+    assert with_workloads == set(mb._CASES)
+    for name in with_workloads:
+        for row in load_manifest()[name]["workloads"]:
+            assert 0 <= mb._kv_gib(row) < 64 and all(d in mb._DT for d in row["dtypes"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op, label, op_module", [
+    ("PagedKVCacheAllocFwdOp", "decode-64-p64", "serving_ops"), ("PagedKVCacheReleaseFwdOp", "release-64-p64", "serving_ops"),
+    ("QKNormRopePagedKVAppendFwdOp", "llama3-8b-decode-fp4kv", "serving_ops"), ("PagedFP4KVCacheGatherFwdOp", "gather-8192", "serving_ops"),
+    ("GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp", "llama3-8b-paged-fp4kv", "serving_ops"),
+])
+def test_serving_step_rows_end_to_end(tmp_path, op, label, op_module):
+    assert mb.main(["--op", op, "--label", label, "--steps", "3", "--out", str(tmp_path)]) == 0
+    (case,) = ET.parse(tmp_path / "junit.xml").getroot().findall("testcase")
+    p = _props(case)
+    assert p["op"] == op and p["op_module"] == f"tileops_amd.{op_module}" and float(p["tileops_latency_ms"]) > 0
+    assert ("tileops_hbm_frac" in p) == ("Attention" in op) and 0 < float(p.get("tileops_hbm_frac", 0.5)) < 1
+    assert label in (tmp_path / "profile_run.log").read_text()
+
+
 @pytest.mark.gpu
 def test_paged_torch_baseline_computes_what_the_op_computes():
     """The baseline that paged rows are compared with (gather by block table, SDPA with a padding mask) agrees with the op

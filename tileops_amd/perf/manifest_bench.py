@@ -11,13 +11,13 @@ and writes both artefacts itself.
 Per workload and implementation (tag) it records ``latency_ms`` (median device time of one call, HIP events, the
 L2/MALL flushed between calls -- the methodology of benchmarks/timing.py:546-585), ``tflops`` and
 ``bandwidth_tbs`` from the op's ``eval_roofline()`` after it has seen the call, and ``hbm_frac`` = bandwidth over
-the 8 TB/s peak.  ``device_busy_ms`` (sum of kernel durations) is taken from the torch profiler when it delivers
+the 8 TB/s peak (the serving-step ops other than attention state no roofline: latency alone).  ``device_busy_ms`` (sum of kernel durations) is taken from the torch profiler when it delivers
 device events, otherwise left out.  Baselines on the same device (no FlashInfer / AITER build is importable in this
 image; the tag slot is there): tag ``torch_sdpa`` = ``F.scaled_dot_product_attention`` for the contiguous op; tag
 ``torch_gather_sdpa`` = for a paged row, two dense ``index_select`` copies of the pages each sequence addresses followed by
 SDPA with a boolean padding mask and ``enable_gqa`` (torch's math path) -- a plain-torch way to do the same job, not a
 tuned kernel, so its ratio says what a user gains over eager torch and nothing about kernel quality.  Rows with an FP8
-cache, several query tokens or a softcap have no device baseline; the run lists them at its end.
+or 4-bit cache, several query tokens or a softcap have no device baseline, nor have the ops around attention; the run lists them at its end.
 """
 
 from __future__ import annotations
@@ -40,10 +40,14 @@ from ..ops import (
     GroupedQueryAttentionMultiTokenDecodePagedWithKVCacheFwdOp, GroupedQueryAttentionPrefillPagedWithKVCacheFwdOp,
 )
 from ..roofline import _distribute_total, gqa_prefill_paged_with_kv_cache_fwd_roofline
+from ..serving_ops import (
+    GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp, PagedFP4KVCacheGatherFwdOp, PagedKVCacheAllocFwdOp, PagedKVCacheReleaseFwdOp,
+    QKNormRopePagedKVAppendFwdOp,
+)
 from ..workloads import FP8, GroupedQueryAttentionDecodePagedWorkload, PagedDecodeConfig, gen_paged_inputs, quantize_kv_per_token
 
 HBM_PEAK_TBS = 8.0
-_DT = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float8_e4m3fn": FP8}
+_DT = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float8_e4m3fn": FP8, "float4_e2m1fn_x2": torch.float4_e2m1fn_x2, "int32": torch.int32}
 
 
 class BenchmarkReport:
@@ -236,9 +240,14 @@ def _device_busy(fn: Callable[[], Any]) -> tuple[Optional[float], Optional[int]]
 
 
 def _result(op: Any, latency_ms: float, busy: tuple[Optional[float], Optional[int]]) -> dict:
-    flops, nbytes = op.eval_roofline()
-    res = {"latency_ms": latency_ms, "tflops": flops / latency_ms / 1e9, "bandwidth_tbs": nbytes / latency_ms / 1e9}
-    res["hbm_frac"] = res["bandwidth_tbs"] / HBM_PEAK_TBS
+    res = {"latency_ms": latency_ms}
+    try:
+        flops, nbytes = op.eval_roofline()
+    except NotImplementedError:  # (the manifest entry names none)
+        pass
+    else:
+        res.update(tflops=flops / latency_ms / 1e9, bandwidth_tbs=nbytes / latency_ms / 1e9)
+        res["hbm_frac"] = res["bandwidth_tbs"] / HBM_PEAK_TBS
     if busy[0] is not None:
         res["device_busy_ms"], res["n_kernels"] = busy[0], busy[1]
         res["gap_ms"] = max(latency_ms - busy[0], 0.0)
@@ -370,12 +379,87 @@ def _prefill_case(row: dict, dtype: torch.dtype, device: torch.device):
     return op, args, None
 
 
+def _pool_case(row: dict, dtype: torch.dtype, device: torch.device, release: bool):
+    """Sequences of random lengths on a permuted pool; every sequence takes one token, or a quarter of them give their pages back."""
+    batch, width, page, pages = row["batch"], row["max_pages_per_req"], row["page_size"], row["num_pages"]
+    lens = torch.randint(0, width * page, (batch,), device=device)
+    perm = torch.randperm(pages, device=device).to(dtype)
+    table = perm[: batch * width].reshape(batch, width).contiguous()
+    free, count = torch.zeros_like(perm), torch.tensor([pages - batch * width], dtype=dtype, device=device)
+    free[: pages - batch * width] = perm[batch * width:]
+    if release:
+        op = PagedKVCacheReleaseFwdOp(batch, width, page, pages)
+        return op, (torch.arange(batch, device=device) % 4 == 0, lens.to(dtype), table, free, count), None
+    return PagedKVCacheAllocFwdOp(batch, width, page, pages), (lens.to(dtype), table, free, count), None
+
+
+def _fp4_pool(pages: int, heads_kv: int, page: int, dim: int, device: torch.device) -> tuple:
+    """K and V codes, K and V scale bytes: any codes, scales of 2^-6 to 1."""
+    codes = [torch.randint(0, 256, (pages, heads_kv, page, dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+    return (*codes, *(torch.randint(121, 128, (pages, heads_kv, page, dim // 32), dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def _append_case(row: dict, dtype: torch.dtype, device: torch.device):
+    tokens, heads, heads_kv, dim, page = (row[n] for n in ("tokens", "heads", "heads_kv", "dim", "page_size"))
+    cache = _DT[row["cache_dtype"]]
+    op = QKNormRopePagedKVAppendFwdOp(heads, heads_kv, dim, page, cache_dtype=cache)
+    qkv = torch.randn(tokens, (heads + 2 * heads_kv) * dim, device=device).to(dtype)
+    rows = [x.unflatten(1, (-1, dim)) for x in qkv.split([heads * dim, heads_kv * dim, heads_kv * dim], 1)]
+    weights = [torch.ones(dim, dtype=dtype, device=device) for _ in range(2)]
+    angle = torch.arange(8192, device=device)[:, None] * 10000.0 ** (-torch.arange(dim // 2, device=device) / (dim // 2))
+    pages = -(-tokens // page)
+    slots = (torch.randperm(pages, device=device)[:, None] * page + torch.arange(page, device=device)).flatten()[:tokens]
+    if cache != torch.float4_e2m1fn_x2:
+        raise ValueError(f"no generator for cache_dtype {row['cache_dtype']}")
+    return op, (*rows, *weights, angle.cos(), angle.sin(), torch.arange(tokens, dtype=torch.int32, device=device) % 8192, slots,
+                *_fp4_pool(pages, heads_kv, page, dim, device)), None
+
+
+def _gather_case(row: dict, dtype: torch.dtype, device: torch.device):
+    tokens, heads_kv, dim, page = (row[n] for n in ("tokens", "heads_kv", "dim", "page_size"))
+    pages = -(-tokens // page)
+    op = PagedFP4KVCacheGatherFwdOp(heads_kv, dim, page, dtype)
+    return op, (*_fp4_pool(pages, heads_kv, page, dim, device), torch.randperm(pages * page, device=device)[:tokens]), None
+
+
+def _paged_fp4_case(row: dict, dtype: torch.dtype, device: torch.device):
+    qs, (n_kv, heads_kv, dim), page = row["q_shape"], row["kv_shape"], row["page_size"]
+    batch, heads, q_len = qs[0], qs[-2], qs[1] if len(qs) == 4 else 1
+    op = GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp(batch, heads, heads_kv, n_kv, dim, page, q_len=q_len, sm_scale=row.get("sm_scale"),
+                                                           softcap=row.get("softcap"))
+    lo, hi = row["seqlen_range"]
+    lens = torch.randint(lo, hi + 1, (batch,), dtype=torch.int32, device=device)
+    width = -(-hi // page)
+    table = torch.randperm(n_kv // page, device=device)[: batch * width].reshape(batch, width).to(torch.int32)
+    op.observe_call(lens)
+    return op, (torch.randn(tuple(qs), device=device).to(dtype), *_fp4_pool(n_kv // page, heads_kv, page, dim, device), lens, table), None
+
+
 _CASES = {
     "GroupedQueryAttentionDecodePagedWithKVCacheFwdOp": lambda r, d, dev: _paged_case(r, d, dev, False),
     "GroupedQueryAttentionMultiTokenDecodePagedWithKVCacheFwdOp": lambda r, d, dev: _paged_case(r, d, dev, True),
     "GroupedQueryAttentionDecodeWithKVCacheFwdOp": _contiguous_case,
     "GroupedQueryAttentionPrefillPagedWithKVCacheFwdOp": _prefill_case,
+    "PagedKVCacheAllocFwdOp": lambda r, d, dev: _pool_case(r, d, dev, False),
+    "PagedKVCacheReleaseFwdOp": lambda r, d, dev: _pool_case(r, d, dev, True),
+    "QKNormRopePagedKVAppendFwdOp": _append_case,
+    "PagedFP4KVCacheGatherFwdOp": _gather_case,
+    "GroupedQueryAttentionDecodePagedWithFP4KVCacheFwdOp": _paged_fp4_case,
 }
+
+
+def _kv_gib(row: dict) -> float:
+    """K and V of a workload as 16-bit rows, 0 where it has none."""
+    if "kv_shape" in row:
+        shape = row["kv_shape"]
+    elif "dim" in row:
+        shape = (row["physical_tokens"] if "physical_tokens" in row else row["tokens"], row["heads_kv"], row["dim"])
+    else:
+        return 0.0
+    elems = 2
+    for s in shape:
+        elems *= s
+    return elems * 2 / 2**30
 
 
 def main(argv: Optional[list[str]] = None) -> int:
@@ -406,11 +490,8 @@ def main(argv: Optional[list[str]] = None) -> int:
                 continue
             for dname in row["dtypes"]:
                 dtype = _DT[dname]
-                kv_elems = 2
-                for s in row.get("kv_shape") or (row["physical_tokens"], row["heads_kv"], row["dim"]):
-                    kv_elems *= s
-                if kv_elems * 2 / 2**30 > args.max_kv_gib:
-                    print(f"skip {op_name} {row['label']} {dname}: K+V of {kv_elems * 2 / 2**30:.1f} GiB", flush=True)
+                if _kv_gib(row) > args.max_kv_gib:
+                    print(f"skip {op_name} {row['label']} {dname}: K+V of {_kv_gib(row):.1f} GiB", flush=True)
                     continue
                 torch.manual_seed(1235)
                 op, inputs, baseline = _CASES[op_name](row, dtype, device)
@@ -421,6 +502,8 @@ def main(argv: Optional[list[str]] = None) -> int:
                 if "q_shape" in row:
                     params = {"label": row["label"], "q_shape": tuple(row["q_shape"]), "kv_shape": tuple(row["kv_shape"]), "dtype": dname,
                               "kv_dtype": row.get("kv_dtype", dname)}
+                elif "total_q" not in row:
+                    params = {"label": row["label"], "dtype": dname, **{k: v for k, v in row.items() if k not in ("label", "dtypes", "page_size")}}
                 else:
                     params = {"label": row["label"], "total_q": row["total_q"], "batch": row["batch"], "heads": row["heads"],
                               "heads_kv": row["heads_kv"], "dim": row["dim"], "dtype": dname, "kv_dtype": row.get("cache_dtype", dname)}
@@ -428,7 +511,9 @@ def main(argv: Optional[list[str]] = None) -> int:
                     params["page_size"] = row["page_size"]
                 report.record(op_name, params, res, "tileops", getattr(kernel, "config", None))
                 entries = [dict(res, tag="tileops", op=op_name, op_module=type(op).__module__)]
-                line = f"{op_name[:40]:40s} {row['label']:28s} {dname:9s} {lat * 1e3:9.1f} us  {res['bandwidth_tbs']:.2f} TB/s ({100 * res['hbm_frac']:.1f}%)"
+                line = f"{op_name[:40]:40s} {row['label']:28s} {dname:9s} {lat * 1e3:9.1f} us"
+                if "hbm_frac" in res:
+                    line += f"  {res['bandwidth_tbs']:.2f} TB/s ({100 * res['hbm_frac']:.1f}%)"
                 if baseline is not None:
                     bl = _time(baseline, flush, max(args.steps // 2, 3))
                     flops, nbytes = op.eval_roofline()
@@ -447,7 +532,7 @@ def main(argv: Optional[list[str]] = None) -> int:
     write_junit(suite, out_dir / "junit.xml")
     report.dump(out_dir / "profile_run.log")
     if no_baseline:
-        print("no device baseline (FP8 cache, several query tokens, softcap or prefill): " + ", ".join(no_baseline))
+        print("no device baseline (FP8 or 4-bit cache, several query tokens, softcap, prefill or no attention): " + ", ".join(no_baseline))
     print(f"{n} workloads -> {out_dir}/junit.xml, {out_dir}/profile_run.log")
     return 0
 

@@ -224,6 +224,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_fp4_kernel(const 
   // Of the two waves on a SIMD the one that was started first goes first: its workgroup is done after 93 us of 130, and the other goes on alone
   // with a unit half used.  So the second half of the workgroups go first until three quarters of their range (32 x 1024 .. 16384 tokens
   // with eight query tokens, whole call: 129 us without, 126 / 124 / 123 / 125 with 4 / 5 / 6 / 7 eighths; calls that wait for memory: 1%).
+  // (That workgroups half a grid apart share a compute unit is how these grids of two per unit are dealt out, not a promise: where they do not,
+  // the priority costs or gains a little time and nothing else.)
   const int first_until = !p.by_sequence && blockIdx.x >= gridDim.x / 2 ? u_begin + (int)((int64_t)(u_end - u_begin) * 3 / 4) : 0;
   const int64_t rows_all = (int64_t)p.heads_kv * p.rows;
   const bool causal = p.causal && p.q_len > 1, softcap = p.cap_log2e > 0.f, large_cap = p.cap_log2e > kLargeCap;

@@ -26,7 +26,7 @@
 //    is lane-local; the only cross-lane traffic is a two-step max/sum over the four 16-lane groups.
 //  * FP8: V bytes are widened to bf16/fp16 on the LDS->register path (v_cvt_scalef32_pk_*_fp8, OCP e4m3fn).  At head
 //    dims 128 and 256 the K bytes are not widened at all: Q.K^T runs on v_mfma_f32_16x16x128_f8f6f4 against the query
-//    row split into two e4m3fn rows (hi + lo, exact for bf16 queries); at head dim 64 K is widened like V.
+//    row split into two e4m3fn rows (hi + lo, exact for bf16 elements down to 2^-9 of the row's largest); at head dim 64 K is widened like V.
 //    The per-token K scale multiplies the score and the V scale multiplies the probability, so no
 //    head_dim-wide multiplies are spent on dequantisation.  Scales ride the same direct-to-LDS pipeline.
 #include <atomic>
@@ -230,8 +230,8 @@ __global__ __launch_bounds__(NW * 64, (SHW > 1 && (D <= 128 || SHW == 8)) ? 2 : 
   constexpr bool F256 = FP8 && G::ROW == 256;   // fp8 with head dim 256: the 16-bit K layout of 256-byte rows, its own V^T layout
   // Q.K^T on the fp8 matrix instruction (one 128-deep step per 128 head elements): the K bytes go in as they are, the query
   // row goes in as two e4m3fn rows hi + lo (hi = the row times a power of two, rounded; lo = what the rounding dropped,
-  // rounded again: exact for bf16 queries, within 2^-8 of every fp16 element) and the power of two multiplies the
-  // softmax exponent.
+  // rounded again: exact for bf16 elements and within 2^-8 of fp16 elements down to 2^-9 of the row's largest; smaller ones are off by 2^-17 of
+  // that one at most) and the power of two multiplies the softmax exponent.
   constexpr bool QK8 = FP8 && D >= 128;
   constexpr int NCH = D / 64;  // QK8: 16-byte chunks of a row per lane (chunk j = head elements [64j + 16g, 64j + 16g + 16))
   constexpr bool SH = SHW > 1;
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(NW * 64, (SHW > 1 && (D <= 128 || SHW == 8)) ? 2 : 
         for (int e = 0; e < 16 * NCH; e++) am = fmaxf(am, fabsf(f[e]));
         am = fmaxf(group_max(am), 1e-30f);  // over the four lanes that share the row
         // scale by a power of two that puts the row maximum in [128, 256): element mantissas are untouched, so the
-        // eight significant bits of a bf16 element are exactly hi (four) + lo (four)
+        // eight significant bits of a bf16 element are hi (four) + lo (four), as far as e4m3's smallest step of 2^-9 reaches
         const uint32_t be = (__float_as_uint(am) >> 23) & 0xffu;  // biased exponent, >= 27
         const float inv = __uint_as_float((261u - be) << 23);     // 2^(7 - e)
         q_scale[rb] = __uint_as_float((be - 7u) << 23);            // 2^(e - 7)

@@ -22,14 +22,14 @@
 // of that one at most; a probability becomes two bf16 (2^-17 of it), because PV then runs at the rate of 16-bit products.  Waves with two blocks of
 // rows and bf16 queries make do with one bf16 (2^-9; the output's own rounding is that large): they are bound by the vector unit, where
 // the second part takes 40 instructions and 18 products a tile (32 x 1024 .. 16384 tokens with eight query tokens: 115 to 123 us, with both 142 to 154; calls with
-// one block: 8 x 131072 tokens 180 / 183 us, 64 ragged 56 / 55, 1 x 300 7.3 / 7.3).  The row's sum is formed of the rounded ones, so that a
+// one block, one part / two: 8 x 131072 tokens 181 / 184 us, 64 ragged 59 / 61, 16 ragged at head dim 256 52 / 53, 4 x 3000 of 64 rows 17.1 / 18.0).  The row's sum is formed of the rounded ones, so that a
 // common error cancels.  All else is fp32.
 //
 // Bound and measured (8 kv heads, dim 128): 64 query heads, 8 x 131072 tokens, 1.14 GB in 179 us, 6.4 TB/s: memory.  32 query heads, 64
 // sequences of 512 .. 8192 tokens, 304 MB in 48 to 52 us, 5.8 to 6.3 TB/s: memory.  64 query heads, 32 sequences of 1024 .. 16384 tokens with
-// eight query tokens and capped scores: 311 MB in 115 to 130 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
+// eight query tokens and capped scores: 311 MB in 116 to 130 us, bound by the vector unit -- per tile of 32 tokens and two row blocks about
 // 250 vector instructions, 48 of them exponentials and reciprocals at half rate, beside 26 matrix instructions.  One sequence of 300
-// tokens: 7.3 us, the chain of loads length, table entry, tile.
+// tokens: 7.2 to 8 us, the chain of loads length, table entry, tile.
 #include <climits>
 #include <type_traits>
 

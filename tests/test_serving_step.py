@@ -974,6 +974,41 @@ def test_fp4_decode_rows_do_not_see_infinities_that_are_masked(dtype, dim, heads
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, dim, heads, heads_kv, q_len, lens", [
+    (BF16, 128, 8, 1, 1, [9000]), (FP16, 128, 8, 1, 1, [1500]), (BF16, 64, 4, 4, 1, [5000, 700]), (FP16, 256, 4, 2, 2, [4000, 0, 300]),
+    (BF16, 128, 32, 8, 3, [3000, 2500, 40, 1000]), (BF16, 64, 64, 8, 8, [600] * 16 + [40] * 4),
+], ids=str)
+def test_fp4_decode_keeps_what_is_not_a_number_through_the_joining_of_ranges(dtype, dim, heads, heads_kv, q_len, lens):
+    """Sequences spread over ranges that a workgroup, a wave or a wave with four rows joins: a query, a key or a value that is not a number spoils the
+    rows that it belongs to, whichever ranges hold it, and no other."""
+    require_gfx950()
+    page = 16
+    case = _attend_case(dim + heads, dtype, dim, heads, heads_kv, page, lens, q_len=q_len, width=25000)
+    q, k, v, ks, vs, lens_t, table = case
+    want = _attend(case, page, q_len, dtype)
+    assert want.isfinite().all()
+    bad = torch.zeros(want.shape, dtype=torch.bool)
+    q2 = q.clone()
+    for b, n in enumerate(lens):
+        if n:
+            q2[b, -1, b % heads, 3], q2[b, -1, (b + 1) % heads, 0] = math.nan, math.inf
+            bad[b, -1, b % heads] = bad[b, -1, (b + 1) % heads] = True
+    got = _attend((q2, *case[1:]), page, q_len, dtype)
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
+    group = heads // heads_kv
+    for token in (0, lens[0] // 2, lens[0] - q_len):
+        h = token % heads_kv
+        at = (table[0, token // page].long(), h, token % page)
+        for scales, columns in ((ks, slice(None)), (vs, slice(32, 64))):
+            mine = scales.clone()
+            mine[at][1] = 255
+            other = (q, k, v, mine, vs, lens_t, table) if scales is ks else (q, k, v, ks, mine, lens_t, table)
+            got, bad = _attend(other, page, q_len, dtype), torch.zeros(want.shape, dtype=torch.bool)
+            bad[0, :, h * group:(h + 1) * group, columns] = True
+            assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad]), (token, columns)
+
+
+@pytest.mark.gpu
 def test_fp4_decode_clamps_lengths_and_page_ids():
     require_gfx950()
     case = _attend_case(4, BF16, 128, 4, 1, 16, [64, 48, 20], width=4)

@@ -863,9 +863,9 @@ __device__ __forceinline__ void merge_rows(const Fp4Params& p, int b, int64_t ro
       W[0] = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; w++) {
-        const float f = fast_exp2(sh->m[w] - ref);
-        if (f != 0.f) {  // (no range, or none with a weight)
-          W[0] += f * sh->w[w];
+        const float f = fast_exp2(sh->m[w] - ref), sum = sh->w[w];
+        if (f != 0.f || sum != sum) {  // (else no range, or none with a weight; ranges of NaN have no maximum)
+          W[0] += f * sum;
           acc[0] += f * *(const f32x4*)&sh->o[w][d0];
         }
       }
